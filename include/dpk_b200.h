@@ -63,7 +63,7 @@ const char* dpk_last_error(void);
  * filled / drained, 103/104 the same for an accumulator in tensor memory, 105 a routing
  * index outside the token range, 106 misaligned shared memory; kernel 1 gemm_mn, 2 gemm_mn
  * on CTA pairs, 3 gemm_k, 4 gemm_k on CTA pairs, 5 prefill attention, 6 decode attention,
- * 7 routing, 9 router + norm, 11 small-M FFN.  The first report wins until it is read.
+ * 7 routing, 9 router + norm, 11 small-M FFN, 13 to 16 the paged cache (below).  The first report wins until it is read.
  * The reference's device code has no counterpart: its waits are unbounded
  * (DynamicPruningKernels/include/attention_prefill/v3/sm12x_causal.cuh:401,535).
  */
@@ -356,6 +356,107 @@ int dpk_rope_append(void* q, void* k, const void* v, const void* cos, const void
                     int64_t cs_batch_stride, void* k_cache, void* v_cache, int B, int T, int Hq,
                     int Hk, int D, int64_t capacity, int64_t past_len, int dtype,
                     int64_t q_token_stride, int64_t kv_token_stride, void* stream);
+
+/* ------------------------------------------------------------- paged KV cache ----
+ *
+ * A pool of P pages of page_size tokens, [P, page_size, Hk, D] for the keys and for the values,
+ * and the state that says who holds which page, all of it device memory of the caller:
+ *   page_table [S, W] int32   page ids of a sequence's tokens, entry j for tokens [j*page_size, ..)
+ *   kv_lens    [S]    int32   tokens of a sequence in the cache, the new ones of a step included
+ *   ref_counts [P]    int32   number of sequences that hold a page, 0 = free
+ *   query_start [S+1] int32   first new token of each sequence in Q / q / k / v; [0] = 0, [S] = the end
+ * The host never reads any of it.  A page id, length or index outside its range is reported in the
+ * status word (code 105; kernel 13 attention on warps, 14 attention on tensor-memory tiles, 15
+ * rotary embedding, 16 pages) and never followed.  No reference counterpart: the reference's cache
+ * is contiguous (WIDE/wrapper/cache.py:10-60).
+ */
+
+/*
+ * Attention of the new tokens over the paged cache, routed by head group like dpk_attn_prefill /
+ * dpk_attn_decode: new token i of the n_s new tokens of sequence s sees keys j <= kv_lens[s] - n_s + i
+ * (causal) or all kv_lens[s] keys.
+ *   Q [N,Hq,D] (q_token_stride), K, V [P,page_size,Hk,D] (page_stride, page_token_stride; K and V
+ *   alike), mask [N,NG] bytes or NULL = every head, O [N,Hq,D] packed.  Strides in elements,
+ *   multiples of 8; 0 = packed.
+ * Rows of O of routed-out heads and of tokens that see no key are zero; rows behind
+ * query_start[S] are left as they are, or zeroed with clear_tail.  What the cache holds behind
+ * kv_lens, in pages no sequence holds, or in keys that a token may not see, has no influence (values
+ * that a token may not see but another new token of its sequence may: finite values only).
+ * max_query_len: an upper bound of n_s.  It chooses the kernel and the size of the workspace; a
+ * sequence with more new tokens than it says is still computed.
+ * Requirements: D in {64,128}, Hq % Hk == 0, Hq/Hk <= 128, Hq % NG == 0, page_size % 8 == 0.
+ */
+size_t dpk_attn_paged_workspace_bytes(int64_t N, int S, int Hq, int Hk, int D, int max_query_len,
+                                      int has_mask);
+int dpk_attn_paged(const void* Q, const void* K, const void* V, const int32_t* page_table,
+                   const int32_t* kv_lens, const int32_t* query_start, const uint8_t* mask, void* O,
+                   int64_t N, int S, int W, int P, int page_size, int Hq, int Hk, int D, int NG,
+                   float scale, int causal, int dtype, int max_query_len, int clear_tail,
+                   int64_t q_token_stride, int64_t page_stride, int64_t page_token_stride,
+                   int64_t table_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Rotary positions with several axes, and the write of the new k and v into the cache's pages.
+ * Rotary pair i of rotary/2 turns by positions[axis(i)][token] * inv_freq[i]; a pair is channels
+ * (i, rotary/2 + i), or (2i, 2i+1) with `neighbours`; channels from `rotary` on pass through; cos
+ * and sin are multiplied by `scale`.
+ *   q [N,Hq,D], k, v [N,Hk,D] with token strides; q_out [N,Hq,D] (may be q); positions [axes,N]
+ *   int32 or (positions_64) int64, axis_stride elements between axes; inv_freq [rotary/2] fp32.
+ *   axis(i): axis_map [rotary/2] int32 on the device, or `sections` (host array of `axes` pair
+ *   counts that sum to rotary/2: the first sections[0] pairs belong to axis 0, and so on).
+ *   With k_pages / v_pages, token t of sequence s goes to cache position
+ *   kv_lens[s] - query_start[s+1] + t; tokens behind query_start[S] are not touched.  Without
+ *   (both NULL), the rotated k is written to k_out [N,Hk,D] packed (may be k) and v is not read.
+ * Angles in fp64, rotation in fp32, one rounding.  D and rotary multiples of 16, up to 8 axes.
+ */
+int dpk_rope_append_paged(const void* q, const void* k, const void* v, void* q_out, void* k_out,
+                          int64_t q_token_stride, int64_t kv_token_stride, int64_t q_out_token_stride,
+                          const void* positions, int64_t axis_stride, int positions_64,
+                          const float* inv_freq, const int32_t* axis_map, const int32_t* sections,
+                          int axes, int rotary, int neighbours, float scale, void* k_pages,
+                          void* v_pages, int64_t page_stride, int64_t page_token_stride,
+                          const int32_t* page_table, int64_t table_stride, const int32_t* kv_lens,
+                          const int32_t* query_start, int N, int S, int W, int P, int page_size,
+                          int Hq, int Hk, int D, int dtype, void* stream);
+
+/*
+ * Pages: bookkeeping on the device, and the bytes it makes move, in every layer of both pools.
+ * Pools: k, v [layers, P, page_size * row_elems] (layer_stride, page_stride in elements, a page
+ * contiguous).  Workspace: dpk_page_workspace_bytes(S or 0, P or 0, n or 0).
+ *
+ * extend: sequence s gets room for add[s] more tokens.  Pages are taken lowest first by the
+ *   sequences in row order.  A partly filled last page that other sequences hold too is copied
+ *   first for each sequence that will write to it -- but if all its holders write, the first of
+ *   them keeps it.  granted[s] = 0, and nothing changes for s, where add[s] < 0, the row of the
+ *   table is too short, the free pages do not last (a sequence that needs none is granted all the
+ *   same), or where it would keep a shared page of which a later holder is not granted a copy.
+ * fork: children[i] (an empty row that no earlier pair names) becomes a second holder of all
+ *   pages of parents[i]; done[i] = 0 and a report in the status word otherwise.
+ * trim: sequence rows[i] is cut to keep[i] tokens (keep NULL: to none) and lets go of the pages
+ *   behind; longer keeps do nothing; of a row that is named twice the first counts.
+ * copy: page dst[i] becomes a copy of page src[i].  Of several pairs with one destination the last
+ *   counts; a pair whose source is another pair's destination is left out and reported.
+ * compact: moves the held pages into [0, live), each hole in ascending order taking the next held
+ *   page behind `live`; rewrites table and ref_counts; live [1] int32 = their number.
+ */
+size_t dpk_page_workspace_bytes(int S, int P, int n);
+int dpk_page_extend(int32_t* page_table, int64_t table_stride, int32_t* kv_lens, int32_t* ref_counts,
+                    int S, int W, int P, int page_size, const int32_t* add, uint8_t* granted, void* k,
+                    void* v, int layers, int64_t layer_stride, int64_t page_stride, int row_elems,
+                    void* workspace, size_t workspace_bytes, void* stream);
+int dpk_page_fork(int32_t* page_table, int64_t table_stride, int32_t* kv_lens, int32_t* ref_counts,
+                  int S, int W, int P, int page_size, const int32_t* parents, const int32_t* children,
+                  int n, uint8_t* done, void* workspace, size_t workspace_bytes, void* stream);
+int dpk_page_trim(int32_t* page_table, int64_t table_stride, int32_t* kv_lens, int32_t* ref_counts,
+                  int S, int W, int P, int page_size, const int32_t* rows, const int32_t* keep, int n,
+                  void* stream);
+int dpk_page_copy(void* k, void* v, int layers, int64_t layer_stride, int64_t page_stride,
+                  int row_elems, int P, int page_size, const int32_t* src, const int32_t* dst, int n,
+                  void* workspace, size_t workspace_bytes, void* stream);
+int dpk_page_compact(void* k, void* v, int layers, int64_t layer_stride, int64_t page_stride,
+                     int row_elems, int32_t* page_table, int64_t table_stride, int32_t* kv_lens,
+                     int32_t* ref_counts, int S, int W, int P, int page_size, int32_t* live,
+                     void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---- tensor parallel: the row-parallel sum fused into the projection ---------------
  *

@@ -1,0 +1,667 @@
+// Attention of new tokens over a paged KV cache: C-ABI entry, work list, joining kernel and the
+// warp-per-range kernel for few rows (sm_100a).
+//
+// For new token i of sequence s (n_s of them, the last of its kv_len[s] tokens) and query head h:
+//     o = sum_j softmax_j(scale q.k_j) v_j   over the keys j <= kv_len[s] - n_s + i   (causal)
+//                                            or j < kv_len[s]                         (not causal)
+// K and V are read through the page table; rows whose head group is routed out, and rows that see
+// no key, are zero.
+//
+// Three launches: paged_plan_kernel cuts the work (dpk_attn_paged.cuh), an attention kernel runs
+// it, paged_join_kernel joins the tiles that several workers shared and writes the zero rows.
+//
+// The attention kernel here gives every WARP a range of 32-key units.  Its tile is 16 rows, so the
+// Hq/Hk heads of up to 16 / (Hq/Hk) new tokens read every K/V byte once; K and V arrive through a
+// private three-stage ring of cp.async (16-byte copies: a page may end anywhere inside a unit, and
+// rows behind the last key are zero-filled, so whatever an unused row of a page holds is never
+// multiplied).  It is bounded by HBM: 4 * D bytes per key against 16 MMA rows.
+#define DPK_KERNEL_ID 13   // thousands digit of the device status word
+#include "dpk_attn_paged.cuh"
+
+namespace dpk {
+
+// ---- the work list -------------------------------------------------------------------------------
+
+constexpr int kPlanThreads = 1024;
+
+__device__ __forceinline__ int plan_scan(int v, int* sh, int& total)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) sh[warp] = x;
+    __syncthreads();
+    if (warp == 0) {
+        int w = lane < warps ? sh[lane] : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += y;
+        }
+        sh[lane] = w;
+    }
+    __syncthreads();
+    total = sh[warps - 1];
+    return x - v + (warp ? sh[warp - 1] : 0);
+}
+
+// New tokens of sequence s, 0 where query_start does not make sense.
+__device__ __forceinline__ int plan_new(const PagedParams& p, int s, int& tok0)
+{
+    tok0 = p.qstart[s];
+    const int end = p.qstart[s + 1];
+    if (tok0 < 0 || end < tok0 || end > p.N) {
+        atomicCAS(p.status, 0, 1000 * DPK_KERNEL_ID + DPK_DEV_BAD_INDEX);
+        tok0 = 0;
+        return 0;
+    }
+    return end - tok0;
+}
+
+// Active rows of every (sequence, KV head), in token order; used where tiles have many rows, so that
+// none of them is spent on a routed-out (token, head).
+__global__ void __launch_bounds__(1024) paged_rows_kernel(const PagedParams p)
+{
+    __shared__ int sh[33];
+    const int s = blockIdx.x, kvh = blockIdx.y;
+    int tok0;
+    const int total_rows = plan_new(p, s, tok0) * p.rep;
+    int32_t* out = p.rows + (static_cast<int64_t>(kvh) * p.N + tok0) * p.rep;
+    int carry = 0;
+    for (int x0 = 0; x0 < total_rows; x0 += blockDim.x) {
+        const int x = x0 + threadIdx.x;
+        int on = 0;
+        if (x < total_rows) {
+            const int i = x / p.rep, head = kvh * p.rep + (x - i * p.rep);
+            on = p.mask[static_cast<int64_t>(tok0 + i) * p.NG + head / p.hpg] != 0;
+        }
+        int t;
+        const int at = carry + plan_scan(on, sh, t);
+        if (on) out[at] = x;
+        carry += t;
+    }
+    if (threadIdx.x == 0) p.row_count[s * p.Hk + kvh] = carry;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedParams p)
+{
+    __shared__ int sh[33];
+    const int tid = threadIdx.x;
+    const int items = p.S * p.Hk;
+    // 1. tiles of every (sequence, KV head)
+    int carry = 0;
+    for (int x0 = 0; x0 < items; x0 += kPlanThreads) {
+        const int x = x0 + tid;
+        int n = 0;
+        if (x < items) {
+            int tok0;
+            const int s = x / p.Hk;
+            const int rows = p.rows ? p.row_count[x] : plan_new(p, s, tok0) * p.rep;
+            n = (rows + p.tile_rows - 1) / p.tile_rows;
+        }
+        int t;
+        const int at = plan_scan(n, sh, t);
+        if (x < items) p.first_tile[x] = carry + at;
+        carry += t;
+    }
+    const int tiles = min(carry, p.max_tiles);
+    __syncthreads();
+    // 2. the visible keys of every tile; tiles without any are dropped
+    int kept = 0, units = 0;
+    for (int t0 = 0; t0 < tiles; t0 += kPlanThreads) {
+        const int t = t0 + tid;
+        int n = 0;
+        PagedTile pt = {};
+        if (t < tiles) {
+            int lo = 0, hi = items - 1;
+            while (lo < hi) {                        // last item that starts at or before t
+                const int mid = (lo + hi + 1) >> 1;
+                if (p.first_tile[mid] <= t) lo = mid;
+                else hi = mid - 1;
+            }
+            pt.seq = lo / p.Hk;
+            pt.kvh = lo - pt.seq * p.Hk;
+            const int fresh = plan_new(p, pt.seq, pt.tok0);
+            const int rows = p.rows ? p.row_count[lo] : fresh * p.rep;
+            pt.m0 = (t - p.first_tile[lo]) * p.tile_rows;
+            pt.rows = min(p.tile_rows, rows - pt.m0);
+            pt.kv_len = p.kv_lens[pt.seq];
+            if (pt.kv_len < 0 || pt.kv_len > static_cast<int64_t>(p.W) * p.page) {
+                atomicCAS(p.status, 0, 1000 * DPK_KERNEL_ID + DPK_DEV_BAD_INDEX);
+                pt.kv_len = 0;
+            }
+            pt.pos0 = pt.kv_len - fresh;
+            pt.kv_end = pt.kv_len;
+            int any = 1;
+            if (p.causal || (p.mask && !p.rows)) {
+                any = 0;
+                int last = -1, head;
+                if (p.rows || !p.mask) {
+                    last = paged_row(p, pt, pt.rows - 1, head);
+                } else {
+                    for (int r = pt.rows - 1; r >= 0 && last < 0; --r) last = paged_row(p, pt, r, head);
+                }
+                any = last >= 0;
+                if (p.causal) pt.kv_end = min(pt.kv_len, pt.pos0 + last + 1);
+            }
+            if (any && pt.kv_end > 0) n = (pt.kv_end + p.unit_keys - 1) / p.unit_keys;
+        }
+        int total, some;
+        const int slot = kept + plan_scan(n > 0, sh, some);
+        const int first = units + plan_scan(n, sh, total);
+        if (n > 0) {
+            p.tile[slot] = pt;
+            p.start[slot] = first;
+        }
+        kept += some;
+        units += total;
+    }
+    if (tid == 0) {
+        p.start[kept] = units;
+        p.head->tiles = kept;
+        p.head->units = units;
+        p.head->range = max((units + p.workers - 1) / p.workers, p.min_range);
+    }
+}
+
+// ---- attention, a range per warp ---------------------------------------------------------------
+
+constexpr int kPwBN = 32;            // keys per unit
+constexpr int kPwStages = 3;
+constexpr int kPwWarps = 4;
+constexpr int kPwRows = 16;
+
+__device__ __forceinline__ void pw_ldsm_x4(uint32_t addr, uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void pw_ldsm_x4_trans(uint32_t addr, uint32_t (&r)[4])
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+template <bool kBf16>
+__device__ __forceinline__ void pw_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    if constexpr (kBf16) {
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+            "{%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    } else {
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+            "{%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+}
+template <int D>
+__device__ __forceinline__ uint32_t pw_off(int r, int c)
+{
+    return static_cast<uint32_t>(r * (D * 2) + ((c ^ (r & 7)) << 4));
+}
+
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(kPwWarps * 32) paged_warp_kernel(const PagedParams p)
+{
+    constexpr int CH = D / 8, KS = D / 16, NT_S = kPwBN / 8, NT_O = D / 8;
+    constexpr int TILE_B = kPwBN * D * 2;
+    constexpr int WARP_B = kPwStages * 2 * TILE_B;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int gid = lane >> 2, t4 = lane & 3;
+    const uint32_t pipe = smem_u32(smem + warp * WARP_B);
+
+    const int tiles = p.head->tiles, units = p.head->units, range = p.head->range;
+    const int worker = blockIdx.x * kPwWarps + warp;
+    if (static_cast<int64_t>(worker) * range >= units) return;
+    const int u_begin = worker * range, u_end = min(units, u_begin + range);
+
+    // ---- loader: two units ahead of the arithmetic, across the ends of tiles -----------------
+    int ld_tile = paged_find_tile(p.start, tiles, u_begin);
+    int ld_unit = u_begin;                         // the unit to be loaded next
+    int ld_first = p.start[ld_tile], ld_next = p.start[ld_tile + 1];
+    PagedTile lt = p.tile[ld_tile];
+    const int first_tile = ld_tile;
+    // this lane's key of the unit: element offset of its row, -1 behind the last visible key
+    auto key_row = [&]() -> int64_t {
+        if (ld_unit >= u_end) return -1;
+        if (ld_unit >= ld_next) {
+            ++ld_tile;
+            lt = p.tile[ld_tile];
+            ld_first = ld_next;
+            ld_next = p.start[ld_tile + 1];
+        }
+        const int key = (ld_unit - ld_first) * kPwBN + lane;
+        if (key >= lt.kv_end) return -1;
+        const int w = key / p.page;
+        const int id = p.table[lt.seq * p.table_stride + w];
+        if (id < 0 || id >= p.P) {
+            atomicCAS(p.status, 0, 1000 * DPK_KERNEL_ID + DPK_DEV_BAD_INDEX);
+            return -1;
+        }
+        return id * p.page_stride + (key - w * p.page) * p.token_stride + lt.kvh * D;
+    };
+    int64_t my_row = key_row();
+    auto load_unit = [&](int stage) {              // issues the copies of ld_unit, then looks up the next
+        if (ld_unit < u_end) {
+            const uint32_t kdst = pipe + stage * 2 * TILE_B;
+#pragma unroll
+            for (int i = 0; i < CH; ++i) {
+                const int x = i * 32 + lane, r = x / CH, c = x % CH;
+                const int64_t row = __shfl_sync(0xffffffffu, my_row, r);
+                const uint32_t n = row >= 0 ? 16u : 0u;
+                const int64_t off = (row >= 0 ? row : 0) * 2 + c * 16;
+                cp_async_16(kdst + pw_off<D>(r, c), p.K + off, n);
+                cp_async_16(kdst + TILE_B + pw_off<D>(r, c), p.V + off, n);
+            }
+            ++ld_unit;
+            my_row = key_row();
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < kPwStages - 1; ++s) load_unit(s);
+
+    // ---- arithmetic ------------------------------------------------------------------------
+    int tile = first_tile;
+    int stage = 0;
+    for (int u = u_begin; u < u_end; ++tile) {
+        const PagedTile t = p.tile[tile];
+        const int t_first = p.start[tile], t_next = p.start[tile + 1];
+        const int seg_end = min(u_end, t_next);
+        // rows gid and gid + 8 of this lane: token (or -1) and the last key they see
+        int head0 = 0, head1 = 0;
+        const int i0 = gid < t.rows ? paged_row(p, t, gid, head0) : -1;
+        const int i1 = gid + 8 < t.rows ? paged_row(p, t, gid + 8, head1) : -1;
+        const int lim0 = i0 < 0 ? -1 : p.causal ? min(t.kv_len - 1, t.pos0 + i0) : t.kv_len - 1;
+        const int lim1 = i1 < 0 ? -1 : p.causal ? min(t.kv_len - 1, t.pos0 + i1) : t.kv_len - 1;
+        uint32_t qf[KS][4];
+        {
+            const uint8_t* q0 = p.Q + ((t.tok0 + max(i0, 0)) * p.q_ts + static_cast<int64_t>(head0) * D) * 2 + t4 * 4;
+            const uint8_t* q1 = p.Q + ((t.tok0 + max(i1, 0)) * p.q_ts + static_cast<int64_t>(head1) * D) * 2 + t4 * 4;
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                qf[ks][0] = i0 >= 0 ? *reinterpret_cast<const uint32_t*>(q0 + ks * 32) : 0u;
+                qf[ks][1] = i1 >= 0 ? *reinterpret_cast<const uint32_t*>(q1 + ks * 32) : 0u;
+                qf[ks][2] = i0 >= 0 ? *reinterpret_cast<const uint32_t*>(q0 + ks * 32 + 16) : 0u;
+                qf[ks][3] = i1 >= 0 ? *reinterpret_cast<const uint32_t*>(q1 + ks * 32 + 16) : 0u;
+            }
+        }
+        float o[NT_O][4];
+#pragma unroll
+        for (int j = 0; j < NT_O; ++j) { o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f; }
+        float mx0 = -INFINITY, mx1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+
+        for (; u < seg_end; ++u) {
+            int fill = stage + kPwStages - 1;
+            if (fill >= kPwStages) fill -= kPwStages;
+            load_unit(fill);
+            cp_async_wait<kPwStages - 1>();
+            __syncwarp();
+            const uint32_t kbase = pipe + stage * 2 * TILE_B, vbase = kbase + TILE_B;
+            const int kv0 = (u - t_first) * kPwBN;
+            float s[NT_S][4];
+#pragma unroll
+            for (int j = 0; j < NT_S; ++j) { s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f; }
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+#pragma unroll
+                for (int jp = 0; jp < NT_S / 2; ++jp) {
+                    uint32_t kf[4];
+                    const int r = jp * 16 + (lane & 7) + (lane >> 4) * 8;
+                    pw_ldsm_x4(kbase + pw_off<D>(r, ks * 2 + ((lane >> 3) & 1)), kf);
+                    pw_mma<kBf16>(s[2 * jp], qf[ks], kf[0], kf[1]);
+                    pw_mma<kBf16>(s[2 * jp + 1], qf[ks], kf[2], kf[3]);
+                }
+            }
+            if (kv0 + kPwBN - 1 > min(lim0, lim1)) {
+#pragma unroll
+                for (int j = 0; j < NT_S; ++j) {
+                    const int k0 = kv0 + j * 8 + 2 * t4;
+                    if (k0 > lim0) s[j][0] = -INFINITY;
+                    if (k0 + 1 > lim0) s[j][1] = -INFINITY;
+                    if (k0 > lim1) s[j][2] = -INFINITY;
+                    if (k0 + 1 > lim1) s[j][3] = -INFINITY;
+                }
+            }
+            float tm0 = -INFINITY, tm1 = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < NT_S; ++j) {
+                tm0 = fmaxf(tm0, fmaxf(s[j][0], s[j][1]));
+                tm1 = fmaxf(tm1, fmaxf(s[j][2], s[j][3]));
+            }
+            tm0 = fmaxf(tm0, __shfl_xor_sync(0xffffffffu, tm0, 1));
+            tm0 = fmaxf(tm0, __shfl_xor_sync(0xffffffffu, tm0, 2));
+            tm1 = fmaxf(tm1, __shfl_xor_sync(0xffffffffu, tm1, 1));
+            tm1 = fmaxf(tm1, __shfl_xor_sync(0xffffffffu, tm1, 2));
+            const float nm0 = fmaxf(mx0, tm0), nm1 = fmaxf(mx1, tm1);
+            const float ref0 = nm0 == -INFINITY ? 0.f : nm0 * p.scale_log2;
+            const float ref1 = nm1 == -INFINITY ? 0.f : nm1 * p.scale_log2;
+            const float corr0 = paged_exp2(mx0 * p.scale_log2 - ref0);
+            const float corr1 = paged_exp2(mx1 * p.scale_log2 - ref1);
+            mx0 = nm0;
+            mx1 = nm1;
+            float rs0 = 0.f, rs1 = 0.f;
+            // P enters the second product in 16 bits, as the tensor core takes it; its sum is taken
+            // of the rounded values, so that the weights still add up to one
+            uint32_t pf[NT_S][2];
+#pragma unroll
+            for (int j = 0; j < NT_S; ++j) {
+                pf[j][0] = pack_half2<kBf16>(paged_exp2(fmaf(s[j][0], p.scale_log2, -ref0)),
+                                             paged_exp2(fmaf(s[j][1], p.scale_log2, -ref0)));
+                pf[j][1] = pack_half2<kBf16>(paged_exp2(fmaf(s[j][2], p.scale_log2, -ref1)),
+                                             paged_exp2(fmaf(s[j][3], p.scale_log2, -ref1)));
+                float x, y;
+                unpack_half2<kBf16>(pf[j][0], x, y);
+                rs0 += x + y;
+                unpack_half2<kBf16>(pf[j][1], x, y);
+                rs1 += x + y;
+            }
+            l0 = l0 * corr0 + rs0;
+            l1 = l1 * corr1 + rs1;
+#pragma unroll
+            for (int j = 0; j < NT_O; ++j) {
+                o[j][0] *= corr0; o[j][1] *= corr0;
+                o[j][2] *= corr1; o[j][3] *= corr1;
+            }
+#pragma unroll
+            for (int kk = 0; kk < kPwBN / 16; ++kk) {
+                const uint32_t af[4] = {pf[2 * kk][0], pf[2 * kk][1], pf[2 * kk + 1][0], pf[2 * kk + 1][1]};
+#pragma unroll
+                for (int jp = 0; jp < NT_O / 2; ++jp) {
+                    uint32_t vf[4];
+                    const int r = kk * 16 + (lane & 7) + ((lane >> 3) & 1) * 8;
+                    pw_ldsm_x4_trans(vbase + pw_off<D>(r, jp * 2 + (lane >> 4)), vf);
+                    pw_mma<kBf16>(o[2 * jp], af, vf[0], vf[1]);
+                    pw_mma<kBf16>(o[2 * jp + 1], af, vf[2], vf[3]);
+                }
+            }
+            __syncwarp();                            // the stage is refilled by the next unit's copies
+            if (++stage == kPwStages) stage = 0;
+        }
+
+        l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
+        l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
+        l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+        if (t_first >= u_begin && t_next <= u_end) {         // the whole tile was this warp's
+            const float inv0 = l0 > 0.f ? 1.f / l0 : 0.f, inv1 = l1 > 0.f ? 1.f / l1 : 0.f;
+            uint8_t* d0 = p.O + ((static_cast<int64_t>(t.tok0 + max(i0, 0)) * p.Hq + head0) * D + 2 * t4) * 2;
+            uint8_t* d1 = p.O + ((static_cast<int64_t>(t.tok0 + max(i1, 0)) * p.Hq + head1) * D + 2 * t4) * 2;
+#pragma unroll
+            for (int j = 0; j < NT_O; ++j) {
+                if (i0 >= 0)
+                    *reinterpret_cast<uint32_t*>(d0 + j * 16) = pack_half2<kBf16>(o[j][0] * inv0, o[j][1] * inv0);
+                if (i1 >= 0)
+                    *reinterpret_cast<uint32_t*>(d1 + j * 16) = pack_half2<kBf16>(o[j][2] * inv1, o[j][3] * inv1);
+            }
+        } else {
+            const int64_t slot = (static_cast<int64_t>(worker) * 2 + (t_first > u_begin ? 1 : 0)) * kPwRows;
+            float* d0 = p.part_o + (slot + gid) * D + 2 * t4;
+            float* d1 = d0 + 8 * D;
+#pragma unroll
+            for (int j = 0; j < NT_O; ++j) {
+                if (gid < t.rows) *reinterpret_cast<float2*>(d0 + j * 8) = make_float2(o[j][0], o[j][1]);
+                if (gid + 8 < t.rows) *reinterpret_cast<float2*>(d1 + j * 8) = make_float2(o[j][2], o[j][3]);
+            }
+            if (t4 == 0) {
+                float* ml = p.part_ml + (slot + gid) * 2;
+                if (gid < t.rows) *reinterpret_cast<float2*>(ml) = make_float2(mx0, l0);
+                if (gid + 8 < t.rows) *reinterpret_cast<float2*>(ml + 16) = make_float2(mx1, l1);
+            }
+        }
+    }
+    cp_async_wait<0>();
+}
+
+// ---- joining -----------------------------------------------------------------------------------
+
+// Block b < workers - 1 looks at the end of worker b's range: if a tile straddles it and this is the
+// tile's first such border, the block joins the tile's parts.  The other blocks write the rows that
+// no unit covers: routed out, without a visible key, and (clear_tail) behind the last sequence.
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p, int join_blocks)
+{
+    const int tid = threadIdx.x;
+    if (static_cast<int>(blockIdx.x) < join_blocks) {
+        const int units = p.head->units, range = p.head->range;
+        const int64_t border = static_cast<int64_t>(blockIdx.x + 1) * range;
+        if (border >= units) return;
+        const int tile = paged_find_tile(p.start, p.head->tiles, static_cast<int>(border));
+        const int first = p.start[tile], end = p.start[tile + 1];
+        const int w0 = first / range, w1 = (end - 1) / range;
+        if (first == border || w0 != static_cast<int>(blockIdx.x)) return;
+        const PagedTile t = p.tile[tile];
+        const int slot0 = first > w0 * range ? 1 : 0;
+        constexpr int kRowsAtOnce = 128 / (D / 4);           // four columns per thread
+        const int c = (tid % (D / 4)) * 4;
+        for (int r = blockIdx.y * kRowsAtOnce + tid / (D / 4); r < t.rows; r += gridDim.y * kRowsAtOnce) {
+            int head;
+            const int i = paged_row(p, t, r, head);
+            if (i < 0) continue;
+            float m = -INFINITY, l = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int w = w0; w <= w1; ++w) {
+                const int64_t slot = (static_cast<int64_t>(w) * 2 + (w == w0 ? slot0 : 0)) * p.tile_rows + r;
+                const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
+                const float4 x = *reinterpret_cast<const float4*>(p.part_o + slot * D + c);
+                if (ml.x == -INFINITY) continue;
+                const float top = fmaxf(m, ml.x);
+                const float a = m == -INFINITY ? 0.f : paged_exp2((m - top) * p.scale_log2);
+                const float b = paged_exp2((ml.x - top) * p.scale_log2);
+                l = l * a + ml.y * b;
+                acc.x = acc.x * a + x.x * b;
+                acc.y = acc.y * a + x.y * b;
+                acc.z = acc.z * a + x.z * b;
+                acc.w = acc.w * a + x.w * b;
+                m = top;
+            }
+            const float inv = l > 0.f ? 1.f / l : 0.f;
+            uint2 out;
+            out.x = pack_half2<kBf16>(acc.x * inv, acc.y * inv);
+            out.y = pack_half2<kBf16>(acc.z * inv, acc.w * inv);
+            *reinterpret_cast<uint2*>(p.O + ((static_cast<int64_t>(t.tok0 + i) * p.Hq + head) * D + c) * 2) = out;
+        }
+        return;
+    }
+    if (blockIdx.y) return;
+    for (int t = blockIdx.x - join_blocks; t < p.N; t += gridDim.x - join_blocks) {
+        const bool tail = p.S == 0 || t >= p.qstart[p.S];
+        int seen = -1;                                       // last key the token sees
+        if (!tail) {
+            int lo = 0, hi = p.S - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (p.qstart[mid] <= t) lo = mid;
+                else hi = mid - 1;
+            }
+            const int len = p.kv_lens[lo];
+            seen = len <= 0 || len > static_cast<int64_t>(p.W) * p.page ? -1
+                   : p.causal ? min(len - 1, len - p.qstart[lo + 1] + t) : len - 1;
+        }
+        if (tail && !p.clear_tail) continue;
+        for (int x = tid; x < p.Hq * (D / 8); x += 128) {
+            const int head = x / (D / 8);
+            const bool dead = tail || seen < 0 ||
+                              (p.mask && p.mask[static_cast<int64_t>(t) * p.NG + head / p.hpg] == 0);
+            if (dead)
+                *reinterpret_cast<uint4*>(p.O + (static_cast<int64_t>(t) * p.Hq * D + x * 8) * 2) =
+                    make_uint4(0, 0, 0, 0);
+        }
+    }
+}
+
+template <int D, bool kBf16>
+static int launch_warp(const PagedParams& p, cudaStream_t s)
+{
+    constexpr size_t smem = size_t(kPwWarps) * kPwStages * 2 * kPwBN * D * 2;
+    DPK_CUDA(cudaFuncSetAttribute(paged_warp_kernel<D, kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    paged_warp_kernel<D, kBf16><<<p.workers / kPwWarps, kPwWarps * 32, smem, s>>>(p);
+    DPK_CUDA(cudaGetLastError());
+    return DPK_OK;
+}
+
+int attn_paged_warp(const PagedParams& p, int D, int dtype, cudaStream_t s)
+{
+    if (D == 64) return dtype == DPK_BF16 ? launch_warp<64, true>(p, s) : launch_warp<64, false>(p, s);
+    return dtype == DPK_BF16 ? launch_warp<128, true>(p, s) : launch_warp<128, false>(p, s);
+}
+
+template <int D, bool kBf16>
+static int launch_join(const PagedParams& p, cudaStream_t s)
+{
+    const int join = p.workers - 1;
+    int zero = p.N;
+    const int cap = sm_count() * 16;
+    if (zero > cap) zero = cap;
+    const int slices = p.tile_rows <= 16 ? 1 : 8;
+    paged_join_kernel<D, kBf16><<<dim3(join + zero, slices), 128, 0, s>>>(p, join);
+    DPK_CUDA(cudaGetLastError());
+    return DPK_OK;
+}
+
+// Which kernel, and how the work is cut, from what the host knows.
+struct PagedShape {
+    bool tc;
+    int tile_rows, unit_keys, workers, min_range;
+    int64_t max_tiles;
+    size_t off_start, off_tile, off_first, off_rows, off_count, off_o, off_ml, bytes;
+};
+
+static PagedShape paged_shape(int64_t N, int S, int Hq, int Hk, int D, int max_query_len, bool has_mask, int sms)
+{
+    PagedShape g;
+    const int rep = Hq / Hk;
+    (void)max_query_len;
+    g.tc = false;
+    g.tile_rows = kPwRows;
+    g.unit_keys = kPwBN;
+    g.workers = sms * kPwWarps;
+    g.min_range = 2;
+    g.max_tiles = int64_t(Hk) * ((N * rep) / g.tile_rows + S);
+    size_t at = 16;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += (bytes + 15) & ~size_t(15);
+        return here;
+    };
+    g.off_tile = take(size_t(g.max_tiles) * sizeof(PagedTile));
+    g.off_start = take(size_t(g.max_tiles + 1) * 4);
+    g.off_first = take(size_t(S) * Hk * 4);
+    g.off_rows = take(g.tc && has_mask ? size_t(Hk) * N * rep * 4 : 0);
+    g.off_count = take(g.tc && has_mask ? size_t(S) * Hk * 4 : 0);
+    g.off_o = take(size_t(g.workers) * 2 * g.tile_rows * D * 4);
+    g.off_ml = take(size_t(g.workers) * 2 * g.tile_rows * 8);
+    g.bytes = at;
+    return g;
+}
+
+static bool paged_sizes_ok(int64_t N, int S, int Hq, int Hk, int D)
+{
+    return N >= 0 && N < (1ll << 31) && S >= 0 && Hq > 0 && Hk > 0 && D > 0 && Hq % Hk == 0;
+}
+
+}  // namespace dpk
+
+using namespace dpk;
+
+extern "C" {
+
+size_t dpk_attn_paged_workspace_bytes(int64_t N, int S, int Hq, int Hk, int D, int max_query_len, int has_mask)
+{
+    if (!paged_sizes_ok(N, S, Hq, Hk, D)) return 0;
+    return paged_shape(N, S, Hq, Hk, D, max_query_len, has_mask != 0, sm_count()).bytes;
+}
+
+int dpk_attn_paged(const void* Q, const void* K, const void* V, const int32_t* page_table,
+                   const int32_t* kv_lens, const int32_t* query_start, const uint8_t* mask, void* O, int64_t N,
+                   int S, int W, int P, int page_size, int Hq, int Hk, int D, int NG, float scale, int causal,
+                   int dtype, int max_query_len, int clear_tail, int64_t q_token_stride, int64_t page_stride,
+                   int64_t page_token_stride, int64_t table_stride, void* workspace, size_t workspace_bytes,
+                   void* stream)
+{
+    DPK_REQUIRE(Q && K && V && O && page_table && kv_lens && query_start, "NULL tensor");
+    DPK_REQUIRE(dtype == DPK_F16 || dtype == DPK_BF16, "dtype must be DPK_F16 or DPK_BF16");
+    DPK_REQUIRE(N >= 0 && N < (1ll << 31) && S >= 0 && W >= 0 && P >= 0 && Hq > 0 && Hk > 0, "bad shape");
+    DPK_REQUIRE(D == 64 || D == 128, "head_dim %d not supported (64 or 128)", D);
+    DPK_REQUIRE(Hq % Hk == 0, "Hq=%d must be a multiple of Hk=%d", Hq, Hk);
+    DPK_REQUIRE(!mask || (NG > 0 && Hq % NG == 0), "Hq=%d must be a multiple of NG=%d", Hq, NG);
+    DPK_REQUIRE(Hq / Hk <= 128, "more than 128 query heads per KV head are not supported");
+    DPK_REQUIRE(page_size > 0 && page_size % 8 == 0, "page_size %d must be a multiple of 8", page_size);
+    DPK_REQUIRE(int64_t(W) * page_size < (1ll << 30), "a row of the table holds 2^30 tokens or more");
+    DPK_REQUIRE(max_query_len >= 1, "max_query_len must be at least 1");
+    const int64_t q_ts = q_token_stride ? q_token_stride : int64_t(Hq) * D;
+    const int64_t kv_ts = page_token_stride ? page_token_stride : int64_t(Hk) * D;
+    const int64_t ps = page_stride ? page_stride : page_size * kv_ts;
+    const int64_t ts = table_stride ? table_stride : W;
+    DPK_REQUIRE(q_ts >= int64_t(Hq) * D && kv_ts >= int64_t(Hk) * D && ts >= W,
+                "strides must cover the heads of a token and the pages of a row");
+    DPK_REQUIRE(q_ts % 8 == 0 && kv_ts % 8 == 0 && ps % 8 == 0, "strides must be multiples of 8 elements (16 bytes)");
+    DPK_REQUIRE(aligned16(Q) && aligned16(K) && aligned16(V) && aligned16(O), "tensors must be 16-byte aligned");
+    if (N == 0) return DPK_OK;
+    const int sms = sm_count();
+    const PagedShape g = paged_shape(N, S, Hq, Hk, D, max_query_len, mask != nullptr, sms);
+    DPK_REQUIRE(g.max_tiles * (int64_t(W) * page_size / g.unit_keys + 1) < (1ll << 31),
+                "too much work for one call: %lld tiles of up to %lld keys", (long long)g.max_tiles,
+                (long long)W * page_size);
+    DPK_REQUIRE(int64_t(Hq) * N < (1ll << 31), "too many rows for one call");
+    DPK_REQUIRE(workspace && workspace_bytes >= g.bytes, "workspace of %zu bytes needed, %zu given", g.bytes,
+                workspace_bytes);
+    DPK_REQUIRE(aligned16(workspace), "workspace must be 16-byte aligned");
+    PagedParams p;
+    p.Q = static_cast<const uint8_t*>(Q);
+    p.K = static_cast<const uint8_t*>(K);
+    p.V = static_cast<const uint8_t*>(V);
+    p.O = static_cast<uint8_t*>(O);
+    p.table = page_table;
+    p.kv_lens = kv_lens;
+    p.qstart = query_start;
+    p.mask = mask;
+    p.q_ts = q_ts; p.page_stride = ps; p.token_stride = kv_ts; p.table_stride = ts;
+    p.N = static_cast<int>(N); p.S = S; p.W = W; p.P = P; p.page = page_size;
+    p.Hq = Hq; p.Hk = Hk; p.NG = mask ? NG : 1;
+    p.rep = Hq / Hk;
+    p.hpg = Hq / p.NG;
+    p.causal = causal ? 1 : 0;
+    p.clear_tail = clear_tail ? 1 : 0;
+    p.scale_log2 = scale * 1.4426950408889634f;
+    uint8_t* w = static_cast<uint8_t*>(workspace);
+    p.head = reinterpret_cast<PagedHead*>(w);
+    p.tile = reinterpret_cast<PagedTile*>(w + g.off_tile);
+    p.start = reinterpret_cast<int32_t*>(w + g.off_start);
+    p.first_tile = reinterpret_cast<int32_t*>(w + g.off_first);
+    p.rows = g.tc && mask ? reinterpret_cast<int32_t*>(w + g.off_rows) : nullptr;
+    p.row_count = g.tc && mask ? reinterpret_cast<int32_t*>(w + g.off_count) : nullptr;
+    p.part_o = reinterpret_cast<float*>(w + g.off_o);
+    p.part_ml = reinterpret_cast<float*>(w + g.off_ml);
+    p.tile_rows = g.tile_rows; p.unit_keys = g.unit_keys;
+    p.workers = g.workers; p.min_range = g.min_range;
+    p.max_tiles = static_cast<int>(g.max_tiles);
+    p.status = device_status_ptr();
+    if (!p.status) return fail(DPK_ERR_CUDA, "no status word on this device");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (p.rows && S > 0) {
+        DPK_REQUIRE(Hk <= 65535, "grid too large");
+        paged_rows_kernel<<<dim3(S, Hk), max_query_len * p.rep > 512 ? 1024 : 128, 0, s>>>(p);
+        DPK_CUDA(cudaGetLastError());
+    }
+    paged_plan_kernel<<<1, kPlanThreads, 0, s>>>(p);
+    DPK_CUDA(cudaGetLastError());
+    int rc = attn_paged_warp(p, D, dtype, s);
+    if (rc) return rc;
+    if (D == 64) return dtype == DPK_BF16 ? launch_join<64, true>(p, s) : launch_join<64, false>(p, s);
+    return dtype == DPK_BF16 ? launch_join<128, true>(p, s) : launch_join<128, false>(p, s);
+}
+
+}  // extern "C"

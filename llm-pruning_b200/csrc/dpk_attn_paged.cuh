@@ -1,0 +1,99 @@
+// Attention of new tokens over a paged cache: what the work list, the two attention kernels and the
+// joining kernel share.
+//
+// The work is cut into TILES and UNITS.  A tile is up to `tile_rows` (new token, query head) rows of
+// one sequence and one KV head; a unit is `unit_keys` consecutive keys of a tile's visible range.
+// The units of all tiles form one line, and worker w (a warp or a CTA) takes units
+// [w * range, (w + 1) * range): sequences of very different lengths load the GPU evenly, a long
+// cache with few rows is split over many workers, and nothing depends on lengths the host does not
+// know.  A tile that one worker covers is finished there; of the others every worker leaves its
+// un-normalised sum, its row maxima and row sums in one of its two slots (slot 0 for the tile that
+// was begun by an earlier worker or starts with the range, slot 1 for the tile that starts later),
+// and the joining kernel adds them in worker order: the same bits on every run.
+#pragma once
+
+#include "dpk_host.h"
+#include "dpk_sm100.cuh"
+
+namespace dpk {
+
+struct PagedTile {
+    int32_t seq, kvh;       // sequence, KV head
+    int32_t m0, rows;       // rows [m0, m0 + rows) of the (sequence, KV head)'s row list
+    int32_t kv_len;         // tokens of the sequence in the cache
+    int32_t kv_end;         // keys [0, kv_end) are visible to some row of the tile
+    int32_t pos0;           // cache position of the sequence's first new token
+    int32_t tok0;           // its index in Q
+};
+
+struct PagedHead {          // written by the planning kernel
+    int32_t tiles;          // tiles with work
+    int32_t units;          // units of all of them
+    int32_t range;          // units per worker
+    int32_t pad;
+};
+
+struct PagedParams {
+    const uint8_t* Q;       // [N, Hq, D]
+    const uint8_t* K;       // [P, page, Hk, D]
+    const uint8_t* V;
+    uint8_t* O;             // [N, Hq, D] packed
+    const int32_t* table;   // [S, W]
+    const int32_t* kv_lens; // [S]
+    const int32_t* qstart;  // [S + 1]
+    const uint8_t* mask;    // [N, NG] or NULL
+    int64_t q_ts, page_stride, token_stride, table_stride;   // elements
+    int N, S, W, P, page, Hq, Hk, NG, rep, hpg;
+    int causal, clear_tail;
+    float scale_log2;
+    // workspace
+    PagedHead* head;
+    int32_t* start;         // [tiles + 1] first unit of each tile
+    PagedTile* tile;        // [tiles]
+    int32_t* first_tile;    // [S * Hk + 1] running number of tiles before dropping empty ones
+    int32_t* rows;          // [Hk][N * rep] active rows of each (sequence, KV head), or NULL: all rows
+    int32_t* row_count;     // [S * Hk] with `rows`
+    float* part_o;          // [workers][2][tile_rows][D]
+    float* part_ml;         // [workers][2][tile_rows][2]
+    int tile_rows, unit_keys, workers, min_range, max_tiles;
+    int* status;
+};
+
+// Row r of a tile's list -> new token and query head; -1 where the row is routed out.
+__device__ __forceinline__ int paged_row(const PagedParams& p, const PagedTile& t, int r, int& head)
+{
+    int x = t.m0 + r;
+    if (p.rows) x = p.rows[(static_cast<int64_t>(t.kvh) * p.N + t.tok0) * p.rep + x];
+    const int i = x / p.rep;
+    head = t.kvh * p.rep + (x - i * p.rep);
+    if (!p.rows && p.mask && p.mask[static_cast<int64_t>(t.tok0 + i) * p.NG + head / p.hpg] == 0) return -1;
+    return i;
+}
+
+// Last tile whose first unit is at or before `unit`; the whole warp searches, 32 probes a step.
+__device__ __forceinline__ int paged_find_tile(const int32_t* start, int tiles, int unit)
+{
+    int lo = 0, hi = tiles;                         // answer in [lo, hi)
+    const int lane = threadIdx.x & 31;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32;
+        const int at = lo + lane * step;
+        const bool ok = at < hi && start[at] <= unit;
+        const int n = __popc(__ballot_sync(0xffffffffu, ok));      // lane 0 always holds
+        hi = min(hi, lo + n * step);
+        lo = lo + (n - 1) * step;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ float paged_exp2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+int attn_paged_warp(const PagedParams& p, int D, int dtype, cudaStream_t s);
+int attn_paged_tc(const PagedParams& p, int D, int dtype, cudaStream_t s);
+
+}  // namespace dpk

@@ -6,7 +6,7 @@ __init__.py:25-89``): ``get_kernel``, ``run_kernel``, ``list_kernels``,
 types.  The four reference families (``gemm_mn``, ``gemm_k``,
 ``attention_prefill``, ``attention_decode``) are registered under the backend name
 ``"b200"`` for architecture ``"sm100"``; ``ffn_swiglu`` is an extra family for the
-fused FFN.  ``install_into(reference_module)`` registers the same callables in the
+fused FFN, ``attention_paged`` one for attention over a paged KV cache.  ``install_into(reference_module)`` registers the same callables in the
 reference's own registry so that ``backend="auto"`` selects them on a B200.
 """
 
@@ -39,6 +39,9 @@ def _register_builtin() -> None:
     register_kernel("ffn_swiglu", BACKEND, "dpk_b200.ops:ffn_swiglu", requires=("torch",),
                     priority=_PRIORITY, description="routing + fused gate/up + down in one call",
                     replace=True)
+    register_kernel("attention_paged", BACKEND, "dpk_b200.ops:attention_paged", variants={0: (ARCH,)},
+                    default_version=0, requires=("torch",), priority=_PRIORITY, replace=True,
+                    description="head-group-routed attention of new tokens over a paged cache")
 
 
 _register_builtin()

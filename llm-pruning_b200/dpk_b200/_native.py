@@ -58,6 +58,22 @@ SIGNATURES = {
                                _i32, _i32, _i32, _i32, _i32, _vp]),
     "dpk_rope_append": (_i32, [_vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i32, _i32, _i32, _i32, _i32,
                                _i64, _i64, _i32, _i64, _i64, _vp]),
+    "dpk_attn_paged_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "dpk_attn_paged": (_i32, [_vp] * 8 + [_i64] + [_i32] * 8 + [_f32] + [_i32] * 4 + [_i64] * 4
+                       + [_vp, _sz, _vp]),
+    "dpk_rope_append_paged": (_i32, [_vp] * 5 + [_i64] * 3 + [_vp, _i64, _i32, _vp, _vp, _vp, _i32, _i32,
+                                     _i32, _f32, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _vp]
+                              + [_i32] * 9 + [_vp]),
+    "dpk_page_workspace_bytes": (_sz, [_i32, _i32, _i32]),
+    "dpk_page_extend": (_i32, [_vp, _i64, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i32,
+                               _i64, _i64, _i32, _vp, _sz, _vp]),
+    "dpk_page_fork": (_i32, [_vp, _i64, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _vp, _vp, _sz,
+                             _vp]),
+    "dpk_page_trim": (_i32, [_vp, _i64, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _vp]),
+    "dpk_page_copy": (_i32, [_vp, _vp, _i32, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _i32, _vp, _sz,
+                             _vp]),
+    "dpk_page_compact": (_i32, [_vp, _vp, _i32, _i64, _i64, _i32, _vp, _i64, _vp, _vp, _i32, _i32, _i32,
+                                _i32, _vp, _vp, _sz, _vp]),
     "dpk_peer_barrier": (_i32, [C.POINTER(_vp), _vp, _i32, _i32, C.c_uint32, _i32, _vp]),
     "dpk_peer_alloc": (_i32, [_sz, C.POINTER(_vp), _vp]),
     "dpk_peer_open": (_i32, [_vp, C.POINTER(_vp)]),

@@ -40,6 +40,9 @@ SOURCES = [
     "dpk_router_norm.cu",
     "dpk_rope.cu",
     "dpk_ffn_small.cu",
+    "dpk_attn_paged.cu",
+    "dpk_rope_paged.cu",
+    "dpk_pages.cu",
 ]
 
 NVCC_FLAGS = [

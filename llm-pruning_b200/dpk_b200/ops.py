@@ -15,6 +15,8 @@ from typing import Dict, Optional, Tuple
 import torch
 
 from . import _native as N
+from .paged import (attention_paged, page_compact, page_copy, page_extend, page_fork,  # noqa: F401
+                    page_trim, rope_append_paged, rope_axes)
 
 _GEMV_MN_MAX_M = 4   # reference: python/gemm_mn/jit.py:41
 

@@ -1,5 +1,5 @@
 // Attention of new tokens over a paged KV cache: C-ABI entry, work list, joining kernel and the
-// warp-per-range kernel for few rows (sm_100a).
+// warp-per-range kernel for few rows (sm_100a).  The kernel for chunks is in dpk_attn_paged_tc.cu.
 //
 // For new token i of sequence s (n_s of them, the last of its kv_len[s] tokens) and query head h:
 //     o = sum_j softmax_j(scale q.k_j) v_j   over the keys j <= kv_len[s] - n_s + i   (causal)
@@ -354,19 +354,18 @@ __global__ void __launch_bounds__(kPwWarps * 32) paged_warp_kernel(const PagedPa
             mx1 = nm1;
             float rs0 = 0.f, rs1 = 0.f;
             // P enters the second product in 16 bits, as the tensor core takes it; its sum is taken
-            // of the rounded values, so that the weights still add up to one
+            // in 32 bits
             uint32_t pf[NT_S][2];
 #pragma unroll
             for (int j = 0; j < NT_S; ++j) {
-                pf[j][0] = pack_half2<kBf16>(paged_exp2(fmaf(s[j][0], p.scale_log2, -ref0)),
-                                             paged_exp2(fmaf(s[j][1], p.scale_log2, -ref0)));
-                pf[j][1] = pack_half2<kBf16>(paged_exp2(fmaf(s[j][2], p.scale_log2, -ref1)),
-                                             paged_exp2(fmaf(s[j][3], p.scale_log2, -ref1)));
-                float x, y;
-                unpack_half2<kBf16>(pf[j][0], x, y);
-                rs0 += x + y;
-                unpack_half2<kBf16>(pf[j][1], x, y);
-                rs1 += x + y;
+                const float p0 = paged_exp2(fmaf(s[j][0], p.scale_log2, -ref0));
+                const float p1 = paged_exp2(fmaf(s[j][1], p.scale_log2, -ref0));
+                const float p2 = paged_exp2(fmaf(s[j][2], p.scale_log2, -ref1));
+                const float p3 = paged_exp2(fmaf(s[j][3], p.scale_log2, -ref1));
+                rs0 += p0 + p1;
+                rs1 += p2 + p3;
+                pf[j][0] = pack_half2<kBf16>(p0, p1);
+                pf[j][1] = pack_half2<kBf16>(p2, p3);
             }
             l0 = l0 * corr0 + rs0;
             l1 = l1 * corr1 + rs1;
@@ -543,11 +542,12 @@ static PagedShape paged_shape(int64_t N, int S, int Hq, int Hk, int D, int max_q
 {
     PagedShape g;
     const int rep = Hq / Hk;
-    (void)max_query_len;
-    g.tc = false;
-    g.tile_rows = kPwRows;
-    g.unit_keys = kPwBN;
-    g.workers = sms * kPwWarps;
+    // up to 16 rows per sequence and KV head are one tile of the warp kernel; more of them would
+    // read K and V once per 16 rows there
+    g.tc = static_cast<int64_t>(max_query_len) * rep > kPwRows;
+    g.tile_rows = g.tc ? 128 : kPwRows;
+    g.unit_keys = g.tc ? 64 : kPwBN;
+    g.workers = g.tc ? 2 * sms : sms * kPwWarps;
     g.min_range = 2;
     g.max_tiles = int64_t(Hk) * ((N * rep) / g.tile_rows + S);
     size_t at = 16;
@@ -658,8 +658,11 @@ int dpk_attn_paged(const void* Q, const void* K, const void* V, const int32_t* p
     }
     paged_plan_kernel<<<1, kPlanThreads, 0, s>>>(p);
     DPK_CUDA(cudaGetLastError());
-    int rc = attn_paged_warp(p, D, dtype, s);
-    if (rc) return rc;
+    // without a page there is nothing to load: every length is 0, and the work list is empty
+    if (P > 0) {
+        const int rc = g.tc ? attn_paged_tc(p, D, dtype, s) : attn_paged_warp(p, D, dtype, s);
+        if (rc) return rc;
+    }
     if (D == 64) return dtype == DPK_BF16 ? launch_join<64, true>(p, s) : launch_join<64, false>(p, s);
     return dtype == DPK_BF16 ? launch_join<128, true>(p, s) : launch_join<128, false>(p, s);
 }

@@ -1,0 +1,436 @@
+// Attention of new tokens over a paged KV cache on tcgen05 tensor cores (sm_100a): chunks of tokens.
+//
+// A CTA is a worker of the work list (dpk_attn_paged.cuh): it walks its range of 64-key units, tile
+// after tile.  A tile is 128 active (token, query head) rows of one sequence and one KV head, so the
+// heads that share K and V share its loads too.  Per unit
+//     S = Q K^T      UMMA 128 x 64 x D, both operands K-major in shared memory, S in TMEM (two buffers)
+//     P = exp2(..)   four warps, one row per thread: running reference maximum and sum in registers,
+//                    P in 16 bits back into TMEM over S
+//     O += P V       UMMA 128 x D x 64, A = P from TMEM, V in its natural [key][d] layout
+// O is rescaled only when a row's maximum has grown by more than 2^8.
+//
+// K and V arrive by TMA through a map [page][row of page][Hk * D] whose box is gcd(page_size, 64) rows
+// by 64 channels: a unit is put together from as many boxes as pages meet in it, each lane of the
+// producer warp looking up and loading its own.  Boxes behind the tile's last visible key get a page
+// number outside the map and arrive as zeros; rows of V behind it inside a box (whatever a page holds
+// behind its sequence) are cleared in shared memory by the softmax warps before the product, since
+// 0 * NaN would not be 0.  Their K needs nothing: those scores are replaced by -inf.
+//
+// Warp roles (192 threads): 0-3 softmax and epilogue, 4 producer, 5 UMMA issuer and TMEM owner.
+// 96 KiB of shared memory and 256 TMEM columns: two CTAs share an SM and fill each other's gaps.
+// All waits are bounded.
+#define DPK_KERNEL_ID 14   // thousands digit of the device status word
+#include "dpk_attn_paged.cuh"
+#include "dpk_attn_tc.cuh"
+
+namespace dpk {
+
+constexpr int kPtBM = 128, kPtBN = 64, kPtThreads = 192, kPtTmemCols = 256;
+constexpr float kPtRescale = 8.0f;       // log2 units
+
+template <int D>
+struct PtSmem {
+    static constexpr int kQ = kPtBM * D * 2, kKV = kPtBN * D * 2;
+    static constexpr int kOffQ = 0, kOffK = kQ, kOffV = kOffK + 2 * kKV, kOffBar = kOffV + 2 * kKV;
+    static constexpr int kTotal = kOffBar + 16 * 8 + 16;
+};
+
+template <int D, bool kBf16>
+__global__ void __launch_bounds__(kPtThreads, 2)
+paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                const PagedParams p, const int box_rows)
+{
+    using L = PtSmem<D>;
+    constexpr int KBQ = D / 64;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t* sQ = smem + L::kOffQ;
+    uint8_t* sK = smem + L::kOffK;
+    uint8_t* sV = smem + L::kOffV;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kOffBar);
+    // one barrier per buffer, so that no role can complete two phases of one before the other looks
+    uint64_t* q_full = bars;
+    uint64_t* k_full = bars + 1;      // [2] each
+    uint64_t* v_full = bars + 3;
+    uint64_t* k_empty = bars + 5;
+    uint64_t* v_empty = bars + 7;
+    uint64_t* s_full = bars + 9;
+    uint64_t* p_full = bars + 11;
+    uint64_t* pv_done = bars + 13;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int units = p.head->units, range = p.head->range;
+    const int worker = blockIdx.x;
+    if (static_cast<int64_t>(worker) * range >= units) return;      // whole CTA: nothing allocated yet
+    if ((smem_u32(smem) & 1023u) != 0u) {
+        if (threadIdx.x == 0) atomicCAS(p.status, 0, 1000 * DPK_KERNEL_ID + DPK_DEV_BAD_SMEM_BASE);
+        return;
+    }
+    const int u_begin = worker * range, u_end = min(units, u_begin + range);
+    const int tile0 = paged_find_tile(p.start, p.head->tiles, u_begin);
+
+    if (warp == 4 && lane == 0) {
+        mbar_init(q_full, 128);
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(&k_full[s], 1);
+            mbar_init(&k_empty[s], 1);
+            mbar_init(&v_full[s], 1);
+            mbar_init(&v_empty[s], 1);
+            mbar_init(&s_full[s], 1);
+            mbar_init(&p_full[s], 128);
+            mbar_init(&pv_done[s], 1);
+        }
+        *abort_flag = 0;
+        mbar_init_fence();
+        tma_prefetch_desc(&tmK);
+        tma_prefetch_desc(&tmV);
+    }
+    if (warp == 5) tmem_alloc(tmem_slot, kPtTmemCols);
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem_base = *tmem_slot;
+    const uint32_t tmem_o = tmem_base + 128;
+
+    if (warp < 4) {
+        // =================== softmax / epilogue: thread = row of the tile ==================
+        const int row = warp * 32 + lane;
+        const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
+        bool alive = true;
+        int it = 0;                                     // units done, over all tiles
+        for (int tile = tile0, u = u_begin; alive && u < u_end; ++tile) {
+            const PagedTile t = p.tile[tile];
+            const int t_first = p.start[tile], t_next = p.start[tile + 1];
+            const int seg_end = min(u_end, t_next);
+            // Q rows into the swizzled K-major layout (8 lanes per 128 bytes, 16 rows per pass).
+            // The scores of the last tile's last unit were waited for: nothing reads the old Q.
+            {
+                const int chunk = threadIdx.x & 7, rsub = threadIdx.x >> 3;
+                for (int r = rsub; r < kPtBM; r += 16) {
+                    int head = 0;
+                    const int i = r < t.rows ? paged_row(p, t, r, head) : -1;
+                    const uint8_t* src = p.Q;
+                    if (i >= 0) src += (static_cast<int64_t>(t.tok0 + i) * p.q_ts + static_cast<int64_t>(head) * D) * 2;
+#pragma unroll
+                    for (int kb = 0; kb < KBQ; ++kb)
+                        cp_async_16(smem_u32(sQ) + kb * (kPtBM * 128) + r * 128 + ((chunk ^ (r & 7)) << 4),
+                                    src + kb * 128 + chunk * 16, i >= 0 ? 16u : 0u);
+                }
+                cp_async_commit();
+            }
+            int head = 0, head0 = 0;
+            const int tok = row < t.rows ? paged_row(p, t, row, head) : -1;
+            const int tok_first = paged_row(p, t, 0, head0);
+            const int lim = tok < 0 ? -1 : p.causal ? min(t.kv_len - 1, t.pos0 + tok) : t.kv_len - 1;
+            // the fewest keys that a row of the tile sees (rows are in token order)
+            const int lim_first = p.causal ? min(t.kv_len - 1, t.pos0 + tok_first) : t.kv_len - 1;
+            const bool idle = warp * 32 >= t.rows;      // none of this warp's rows exists
+            cp_async_wait<0>();
+            fence_proxy_async_smem();
+            mbar_arrive(q_full);
+
+            float m_ref = -INFINITY, l_sum = 0.f;
+            const int seg_it = it;
+            for (; u < seg_end; ++u, ++it) {
+                const int sb = it & 1;
+                const uint32_t ph = (it >> 1) & 1;
+                const bool got = mbar_wait(&s_full[sb], ph, abort_flag, p.status, DPK_DEV_TIMEOUT_TMEM_FULL);
+                if (!__all_sync(0xffffffffu, got)) { alive = false; break; }
+                tc_fence_after_sync();
+                const int kv0 = (u - t_first) * kPtBN;
+                if (kv0 + kPtBN > t.kv_end && t.kv_end % box_rows != 0) {
+                    // rows of V behind the last visible key that arrived with their box
+                    const bool ok = mbar_wait(&v_full[sb], ph, abort_flag, p.status, DPK_DEV_TIMEOUT_FULL);
+                    if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
+                    const int r0 = t.kv_end - kv0;
+                    const int r1 = min(kPtBN, (r0 + box_rows - 1) / box_rows * box_rows);
+                    uint8_t* v = sV + sb * L::kKV;
+                    for (int x = threadIdx.x; x < (r1 - r0) * KBQ * 8; x += 128) {
+                        const int r = r0 + x / (KBQ * 8), c = x % (KBQ * 8);
+                        *reinterpret_cast<uint4*>(v + (c >> 3) * (kPtBN * 128) + r * 128 + (c & 7) * 16) =
+                            make_uint4(0, 0, 0, 0);
+                    }
+                    fence_proxy_async_smem();
+                }
+                if (idle) {
+                    tc_fence_before_sync();
+                    mbar_arrive(&p_full[sb]);
+                    continue;
+                }
+                const uint32_t ts = tmem_base + sb * kPtBN + lane_base;
+                uint32_t sv[kPtBN];
+                {
+                    uint32_t a32[32], b32[32];
+                    tmem_ld_32x32b_x32(ts, a32);
+                    tmem_ld_32x32b_x32(ts + 32, b32);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) { sv[i] = a32[i]; sv[32 + i] = b32[i]; }
+                }
+                if (kv0 + kPtBN - 1 > lim_first) {
+#pragma unroll
+                    for (int i = 0; i < kPtBN; ++i)
+                        if (kv0 + i > lim) sv[i] = __float_as_uint(-INFINITY);
+                }
+                float t0 = -INFINITY, t1 = -INFINITY, t2 = -INFINITY, t3 = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < kPtBN; i += 8) {
+                    t0 = tc_max3(t0, __uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
+                    t1 = tc_max3(t1, __uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3]));
+                    t2 = tc_max3(t2, __uint_as_float(sv[i + 4]), __uint_as_float(sv[i + 5]));
+                    t3 = tc_max3(t3, __uint_as_float(sv[i + 6]), __uint_as_float(sv[i + 7]));
+                }
+                const float tmax = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3));
+                float alpha = 1.f;
+                bool moved = false;
+                if (tmax > -INFINITY) {
+                    if (m_ref == -INFINITY) {
+                        m_ref = tmax;                   // nothing accumulated yet for this row
+                    } else if ((tmax - m_ref) * p.scale_log2 > kPtRescale) {
+                        alpha = tc_exp2((m_ref - tmax) * p.scale_log2);
+                        m_ref = tmax;
+                        moved = true;
+                    }
+                }
+                const float ref = m_ref == -INFINITY ? 0.f : m_ref * p.scale_log2;
+                // P goes to the second product in 16 bits, as the tensor core takes it; the row sum
+                // is taken in 32 bits
+                uint32_t pk[kPtBN / 2];
+                const float2 sc2 = make_float2(p.scale_log2, p.scale_log2);
+                const float2 nref2 = make_float2(-ref, -ref);
+                float2 ra = make_float2(0.f, 0.f), rb = make_float2(0.f, 0.f);
+#pragma unroll
+                for (int i = 0; i < kPtBN; i += 4) {
+                    const float2 a = __ffma2_rn(make_float2(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1])),
+                                                sc2, nref2);
+                    const float2 b = __ffma2_rn(make_float2(__uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3])),
+                                                sc2, nref2);
+                    const float2 pa = make_float2(tc_exp2(a.x), tc_exp2(a.y));
+                    const float2 pb = make_float2(tc_exp2(b.x), tc_exp2(b.y));
+                    ra = __fadd2_rn(ra, pa);
+                    rb = __fadd2_rn(rb, pb);
+                    pk[i >> 1] = pack_half2<kBf16>(pa.x, pa.y);
+                    pk[(i >> 1) + 1] = pack_half2<kBf16>(pb.x, pb.y);
+                }
+                l_sum = l_sum * alpha + ((ra.x + ra.y) + (rb.x + rb.y));
+                if (it > seg_it && __any_sync(0xffffffffu, moved)) {
+                    // O may only be rescaled once the previous P V has finished
+                    const int pb = (it - 1) & 1;
+                    const bool ok = mbar_wait(&pv_done[pb], ((it - 1) >> 1) & 1, abort_flag, p.status,
+                                              DPK_DEV_TIMEOUT_TMEM_EMPTY);
+                    if (!__all_sync(0xffffffffu, ok)) { alive = false; break; }
+                    tc_fence_after_sync();
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 32) {
+                        uint32_t v[32];
+                        tmem_ld_32x32b_x32(tmem_o + lane_base + c, v);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * alpha);
+                        tmem_st_32x32b_x32(tmem_o + lane_base + c, v);
+                    }
+                    tmem_st_wait();
+                }
+                tmem_st_p(ts, pk);
+                tmem_st_wait();
+                tc_fence_before_sync();
+                mbar_arrive(&p_full[sb]);
+            }
+            if (!alive) break;
+
+            // ---- epilogue: the row, finished or as this worker's part ----------------------
+            const int pb = (it - 1) & 1;
+            const bool ok = mbar_wait(&pv_done[pb], ((it - 1) >> 1) & 1, abort_flag, p.status,
+                                      DPK_DEV_TIMEOUT_TMEM_EMPTY);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            tc_fence_after_sync();
+            if (!idle) {
+                const bool whole = t_first >= u_begin && t_next <= u_end;
+                const float inv = l_sum > 0.f ? 1.f / l_sum : 0.f;
+                const int64_t slot = (static_cast<int64_t>(worker) * 2 + (t_first > u_begin ? 1 : 0)) * kPtBM + row;
+                uint8_t* out = p.O + (static_cast<int64_t>(t.tok0 + max(tok, 0)) * p.Hq + head) * (D * 2);
+#pragma unroll 1
+                for (int c = 0; c < D; c += 32) {
+                    uint32_t v[32];
+                    tmem_ld_32x32b_x32(tmem_o + lane_base + c, v);
+                    tmem_ld_wait();
+                    if (tok < 0) continue;
+                    if (whole) {
+#pragma unroll
+                        for (int q4 = 0; q4 < 4; ++q4) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                w[i] = pack_half2<kBf16>(__uint_as_float(v[q4 * 8 + 2 * i]) * inv,
+                                                         __uint_as_float(v[q4 * 8 + 2 * i + 1]) * inv);
+                            *reinterpret_cast<uint4*>(out + (c + q4 * 8) * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    } else {
+                        float* dst = p.part_o + slot * D + c;
+#pragma unroll
+                        for (int q4 = 0; q4 < 8; ++q4)
+                            *reinterpret_cast<uint4*>(dst + q4 * 4) =
+                                make_uint4(v[q4 * 4], v[q4 * 4 + 1], v[q4 * 4 + 2], v[q4 * 4 + 3]);
+                    }
+                }
+                if (!whole && tok >= 0) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(m_ref, l_sum);
+            }
+            tc_fence_before_sync();     // the next tile's first P V overwrites O after these reads
+        }
+    } else if (warp == 4) {
+        // =================== producer: lane b loads box b of every unit ===================
+        const int boxes = kPtBN / box_rows;
+        const uint32_t box_bytes = box_rows * 128;
+        int tile = tile0, u = u_begin;
+        PagedTile t = p.tile[tile];
+        int t_first = p.start[tile], t_next = p.start[tile + 1];
+        // page and row of this lane's box of the next unit; a page outside the map reads as zeros
+        int next_page = p.P, next_row = 0, next_col = 0;
+        auto look_up = [&]() {
+            next_page = p.P;
+            next_row = 0;
+            if (u >= u_end) return;
+            if (u >= t_next) {
+                ++tile;
+                t = p.tile[tile];
+                t_first = t_next;
+                t_next = p.start[tile + 1];
+            }
+            next_col = t.kvh * D;
+            const int key = (u - t_first) * kPtBN + lane * box_rows;
+            ++u;
+            if (lane >= boxes || key >= t.kv_end) return;
+            const int w = key / p.page;
+            const int id = p.table[t.seq * p.table_stride + w];
+            if (id < 0 || id >= p.P) {
+                atomicCAS(p.status, 0, 1000 * DPK_KERNEL_ID + DPK_DEV_BAD_INDEX);
+                return;
+            }
+            next_page = id;
+            next_row = key - w * p.page;
+        };
+        look_up();
+        const int n = u_end - u_begin;
+        int v_page = 0, v_row = 0, v_col = 0;           // the unit whose V is loaded next
+        bool live = true;
+        // K runs one unit ahead of V: it is needed one softmax earlier and released earlier
+        for (int j = 0; live && j <= n; ++j) {
+            const int k_page = next_page, k_row = next_row, k_col = next_col;
+            if (j < n) {
+                look_up();
+                const int s = j & 1;
+                live = mbar_wait(&k_empty[s], ((j >> 1) & 1) ^ 1, abort_flag, p.status, DPK_DEV_TIMEOUT_EMPTY);
+                live = __all_sync(0xffffffffu, live);
+                if (!live) break;
+                if (lane == 0) mbar_arrive_expect_tx(&k_full[s], L::kKV);
+                __syncwarp();
+                if (lane < boxes) {
+#pragma unroll
+                    for (int kb = 0; kb < KBQ; ++kb)
+                        tma_load_3d(sK + s * L::kKV + kb * (kPtBN * 128) + lane * box_bytes, &tmK, &k_full[s],
+                                    k_col + kb * 64, k_row, k_page);
+                }
+            }
+            if (j > 0) {
+                const int s = (j - 1) & 1;
+                live = mbar_wait(&v_empty[s], (((j - 1) >> 1) & 1) ^ 1, abort_flag, p.status, DPK_DEV_TIMEOUT_EMPTY);
+                live = __all_sync(0xffffffffu, live);
+                if (!live) break;
+                if (lane == 0) mbar_arrive_expect_tx(&v_full[s], L::kKV);
+                __syncwarp();
+                if (lane < boxes) {
+#pragma unroll
+                    for (int kb = 0; kb < KBQ; ++kb)
+                        tma_load_3d(sV + s * L::kKV + kb * (kPtBN * 128) + lane * box_bytes, &tmV, &v_full[s],
+                                    v_col + kb * 64, v_row, v_page);
+                }
+            }
+            v_page = k_page;
+            v_row = k_row;
+            v_col = k_col;
+        }
+    } else {
+        // =================== UMMA issuer ===================================================
+        if (lane == 0) {
+            const uint32_t idesc_s = umma_idesc_f16(kBf16 ? 1 : 0, kPtBM, kPtBN);
+            const uint32_t idesc_o = umma_idesc_f16(kBf16 ? 1 : 0, kPtBM, D) | (1u << 16);   // B is MN-major
+            bool ok = true;
+            int it = 0, seg = 0;
+            for (int tile = tile0, u = u_begin; ok && u < u_end; ++tile, ++seg) {
+                const int len = min(u_end, p.start[tile + 1]) - u;
+                u += len;
+                ok = mbar_wait(q_full, seg & 1, abort_flag, p.status, DPK_DEV_TIMEOUT_FULL);
+                auto issue_s = [&](int i) -> bool {
+                    const int s = i & 1;
+                    if (!mbar_wait(&k_full[s], (i >> 1) & 1, abort_flag, p.status, DPK_DEV_TIMEOUT_FULL)) return false;
+                    tc_fence_after_sync();
+#pragma unroll
+                    for (int kb = 0; kb < KBQ; ++kb) {
+                        const uint64_t a = umma_desc_k_sw128(smem_u32(sQ) + kb * (kPtBM * 128));
+                        const uint64_t b = umma_desc_k_sw128(smem_u32(sK) + s * L::kKV + kb * (kPtBN * 128));
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            umma_f16_ss(tmem_base + s * kPtBN, a + 2 * k, b + 2 * k, idesc_s, (kb | k) != 0 ? 1u : 0u);
+                    }
+                    umma_commit(&s_full[s]);
+                    umma_commit(&k_empty[s]);
+                    return true;
+                };
+                for (int j = 0; ok && j < 2 && j < len; ++j) ok = issue_s(it + j);
+                for (int j = 0; ok && j < len; ++j, ++it) {
+                    const int s = it & 1;
+                    const uint32_t ph = (it >> 1) & 1;
+                    ok = mbar_wait(&p_full[s], ph, abort_flag, p.status, DPK_DEV_TIMEOUT_FULL) &&
+                         mbar_wait(&v_full[s], ph, abort_flag, p.status, DPK_DEV_TIMEOUT_FULL);
+                    if (!ok) break;
+                    tc_fence_after_sync();
+#pragma unroll
+                    for (int k = 0; k < kPtBN / 16; ++k) {
+                        const uint64_t b = umma_desc_mn_sw128(smem_u32(sV) + s * L::kKV + k * 2048, kPtBN * 128);
+                        umma_f16_ts(tmem_o, tmem_base + s * kPtBN + k * 8, b, idesc_o, (j | k) != 0 ? 1u : 0u);
+                    }
+                    umma_commit(&pv_done[s]);
+                    umma_commit(&v_empty[s]);
+                    if (j + 2 < len) ok = issue_s(it + 2);
+                }
+            }
+        }
+    }
+
+    // after a wait that ran out: let copies in flight land before the shared memory goes away
+    if (*abort_flag) __nanosleep(2000000);
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 5) {
+        __syncwarp();
+        tc_fence_after_sync();
+        tmem_dealloc(tmem_base, kPtTmemCols);
+    }
+}
+
+template <int D, bool kBf16>
+static int launch_tc(const PagedParams& p, cudaStream_t s)
+{
+    int box = 64;                                       // gcd(page, 64): page is a multiple of 8
+    while (p.page % box) box >>= 1;
+    CUtensorMap tmK, tmV;
+    const uint64_t cols = static_cast<uint64_t>(p.Hk) * D;
+    int rc = make_tmap_3d_sw128(&tmK, p.K, cols, p.page, p.P, p.token_stride, p.page_stride, 64, box);
+    if (rc) return rc;
+    rc = make_tmap_3d_sw128(&tmV, p.V, cols, p.page, p.P, p.token_stride, p.page_stride, 64, box);
+    if (rc) return rc;
+    constexpr int smem = PtSmem<D>::kTotal;
+    DPK_CUDA(cudaFuncSetAttribute(paged_tc_kernel<D, kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    paged_tc_kernel<D, kBf16><<<p.workers, kPtThreads, smem, s>>>(tmK, tmV, p, box);
+    DPK_CUDA(cudaGetLastError());
+    return DPK_OK;
+}
+
+int attn_paged_tc(const PagedParams& p, int D, int dtype, cudaStream_t s)
+{
+    if (D == 64) return dtype == DPK_BF16 ? launch_tc<64, true>(p, s) : launch_tc<64, false>(p, s);
+    return dtype == DPK_BF16 ? launch_tc<128, true>(p, s) : launch_tc<128, false>(p, s);
+}
+
+}  // namespace dpk

@@ -41,6 +41,7 @@ SOURCES = [
     "dpk_rope.cu",
     "dpk_ffn_small.cu",
     "dpk_attn_paged.cu",
+    "dpk_attn_paged_tc.cu",
     "dpk_rope_paged.cu",
     "dpk_pages.cu",
 ]

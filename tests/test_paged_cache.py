@@ -3,7 +3,7 @@
 Tolerances, per element.  With u half a unit in the last place of the type relative to the value:
 
 * attention: the output is rounded once (u |o|), the weights p are rounded once before the second
-  product and their sum is taken of the rounded ones (u sum p|v|); everything else is in 32 bits:
+  product (u sum p|v|; their sum is taken before); everything else is in 32 bits:
   scores and exponentials are off by less than 2^-13 of a weight here (scores of a few units,
   128 products of 2^-24 each, an exponential of 2^-22).
 * rotation: one rounding (u |x|) and 32-bit sines, cosines and products (2^-20 of |a| + |b|).

@@ -8,7 +8,8 @@
 // no key, are zero.
 //
 // Three launches: paged_plan_kernel cuts the work (dpk_attn_paged.cuh), an attention kernel runs
-// it, paged_join_kernel joins the tiles that several workers shared and writes the zero rows.
+// it, paged_join_kernel joins the tiles that several workers shared and writes the zero rows.  Each
+// is started while its predecessor still runs.
 //
 // The attention kernel here gives every WARP a range of 32-key units.  Its tile is 16 rows, so the
 // Hq/Hk heads of up to 16 / (Hq/Hk) new tokens read every K/V byte once; K and V arrive through a
@@ -23,6 +24,7 @@ namespace dpk {
 // ---- the work list -------------------------------------------------------------------------------
 
 constexpr int kPlanThreads = 1024;
+constexpr int kPlanItems = 4096;        // (sequence, KV head) pairs whose tile numbers fit shared memory
 
 __device__ __forceinline__ int plan_scan(int v, int* sh, int& total)
 {
@@ -64,25 +66,34 @@ __device__ __forceinline__ int plan_new(const PagedParams& p, int s, int& tok0)
 }
 
 // Active rows of every (sequence, KV head), in token order; used where tiles have many rows, so that
-// none of them is spent on a routed-out (token, head).
+// none of them is spent on a routed-out (token, head).  A thread looks at 16 rows in a row.
 __global__ void __launch_bounds__(1024) paged_rows_kernel(const PagedParams p)
 {
     __shared__ int sh[33];
+    paged_let_next_start();
     const int s = blockIdx.x, kvh = blockIdx.y;
     int tok0;
     const int total_rows = plan_new(p, s, tok0) * p.rep;
     int32_t* out = p.rows + (static_cast<int64_t>(kvh) * p.N + tok0) * p.rep;
     int carry = 0;
-    for (int x0 = 0; x0 < total_rows; x0 += blockDim.x) {
-        const int x = x0 + threadIdx.x;
-        int on = 0;
+    for (int x0 = 0; x0 < total_rows; x0 += blockDim.x * 16) {
+        const int x = x0 + threadIdx.x * 16;
+        uint32_t on = 0;
         if (x < total_rows) {
-            const int i = x / p.rep, head = kvh * p.rep + (x - i * p.rep);
-            on = p.mask[static_cast<int64_t>(tok0 + i) * p.NG + head / p.hpg] != 0;
+            int i = x / p.rep, r = x - i * p.rep;
+            const uint8_t* m = p.mask + static_cast<int64_t>(tok0 + i) * p.NG;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                if (x + k < total_rows && m[(kvh * p.rep + r) / p.hpg] != 0) on |= 1u << k;
+                if (++r == p.rep) {
+                    r = 0;
+                    m += p.NG;
+                }
+            }
         }
         int t;
-        const int at = carry + plan_scan(on, sh, t);
-        if (on) out[at] = x;
+        int at = carry + plan_scan(__popc(on), sh, t);
+        for (; on; on &= on - 1) out[at++] = x + __ffs(on) - 1;
         carry += t;
     }
     if (threadIdx.x == 0) p.row_count[s * p.Hk + kvh] = carry;
@@ -91,11 +102,15 @@ __global__ void __launch_bounds__(1024) paged_rows_kernel(const PagedParams p)
 __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedParams p)
 {
     __shared__ int sh[33];
-    const int tid = threadIdx.x;
+    __shared__ int sh_first[kPlanItems];
+    const int tid = threadIdx.x, threads = blockDim.x;
     const int items = p.S * p.Hk;
+    int* first = items <= kPlanItems ? sh_first : p.first_tile;
+    paged_let_next_start();
+    if (p.rows) paged_wait_previous();
     // 1. tiles of every (sequence, KV head)
     int carry = 0;
-    for (int x0 = 0; x0 < items; x0 += kPlanThreads) {
+    for (int x0 = 0; x0 < items; x0 += threads) {
         const int x = x0 + tid;
         int n = 0;
         if (x < items) {
@@ -106,14 +121,14 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedPar
         }
         int t;
         const int at = plan_scan(n, sh, t);
-        if (x < items) p.first_tile[x] = carry + at;
+        if (x < items) first[x] = carry + at;
         carry += t;
     }
     const int tiles = min(carry, p.max_tiles);
     __syncthreads();
     // 2. the visible keys of every tile; tiles without any are dropped
-    int kept = 0, units = 0;
-    for (int t0 = 0; t0 < tiles; t0 += kPlanThreads) {
+    int kept = 0, length = 0;
+    for (int t0 = 0; t0 < tiles; t0 += threads) {
         const int t = t0 + tid;
         int n = 0;
         PagedTile pt = {};
@@ -121,14 +136,14 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedPar
             int lo = 0, hi = items - 1;
             while (lo < hi) {                        // last item that starts at or before t
                 const int mid = (lo + hi + 1) >> 1;
-                if (p.first_tile[mid] <= t) lo = mid;
+                if (first[mid] <= t) lo = mid;
                 else hi = mid - 1;
             }
             pt.seq = lo / p.Hk;
             pt.kvh = lo - pt.seq * p.Hk;
             const int fresh = plan_new(p, pt.seq, pt.tok0);
             const int rows = p.rows ? p.row_count[lo] : fresh * p.rep;
-            pt.m0 = (t - p.first_tile[lo]) * p.tile_rows;
+            pt.m0 = (t - first[lo]) * p.tile_rows;
             pt.rows = min(p.tile_rows, rows - pt.m0);
             pt.kv_len = p.kv_lens[pt.seq];
             if (pt.kv_len < 0 || pt.kv_len > static_cast<int64_t>(p.W) * p.page) {
@@ -153,19 +168,19 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedPar
         }
         int total, some;
         const int slot = kept + plan_scan(n > 0, sh, some);
-        const int first = units + plan_scan(n, sh, total);
+        const int place = length + plan_scan(n > 0 ? n + p.tile_gap : 0, sh, total);
         if (n > 0) {
             p.tile[slot] = pt;
-            p.start[slot] = first;
+            p.start[slot] = place;
         }
         kept += some;
-        units += total;
+        length += total;
     }
     if (tid == 0) {
-        p.start[kept] = units;
+        p.start[kept] = length;
         p.head->tiles = kept;
-        p.head->units = units;
-        p.head->range = max((units + p.workers - 1) / p.workers, p.min_range);
+        p.head->length = length;
+        p.head->range = max((length + p.workers - 1) / p.workers, p.min_range);
     }
 }
 
@@ -222,27 +237,30 @@ __global__ void __launch_bounds__(kPwWarps * 32) paged_warp_kernel(const PagedPa
     const int gid = lane >> 2, t4 = lane & 3;
     const uint32_t pipe = smem_u32(smem + warp * WARP_B);
 
-    const int tiles = p.head->tiles, units = p.head->units, range = p.head->range;
+    paged_wait_previous();
+    paged_let_next_start();
+    const int tiles = p.head->tiles, length = p.head->length, range = p.head->range;
     const int worker = blockIdx.x * kPwWarps + warp;
-    if (static_cast<int64_t>(worker) * range >= units) return;
-    const int u_begin = worker * range, u_end = min(units, u_begin + range);
+    if (static_cast<int64_t>(worker) * range >= length) return;
+    const int u_begin = worker * range, u_end = min(length, u_begin + range);
+    const int tile0 = paged_find_tile(p, tiles, u_begin);
 
     // ---- loader: two units ahead of the arithmetic, across the ends of tiles -----------------
-    int ld_tile = paged_find_tile(p.start, tiles, u_begin);
-    int ld_unit = u_begin;                         // the unit to be loaded next
-    int ld_first = p.start[ld_tile], ld_next = p.start[ld_tile + 1];
-    PagedTile lt = p.tile[ld_tile];
-    const int first_tile = ld_tile;
+    int ld_tile = tile0 - 1, ld_j = 0, ld_n = 0;   // ld_j: the unit of ld_tile to be loaded next
+    PagedTile lt;
+    bool ld_more = true;
     // this lane's key of the unit: element offset of its row, -1 behind the last visible key
     auto key_row = [&]() -> int64_t {
-        if (ld_unit >= u_end) return -1;
-        if (ld_unit >= ld_next) {
+        if (ld_j >= ld_n) {
             ++ld_tile;
+            const int first = ld_tile < tiles ? p.start[ld_tile] : length;
+            ld_more = first < u_end;
+            if (!ld_more) return -1;
             lt = p.tile[ld_tile];
-            ld_first = ld_next;
-            ld_next = p.start[ld_tile + 1];
+            ld_j = max(0, u_begin - first);
+            ld_n = min((lt.kv_end + kPwBN - 1) / kPwBN, u_end - first);
         }
-        const int key = (ld_unit - ld_first) * kPwBN + lane;
+        const int key = ld_j * kPwBN + lane;
         if (key >= lt.kv_end) return -1;
         const int w = key / p.page;
         const int id = p.table[lt.seq * p.table_stride + w];
@@ -254,7 +272,7 @@ __global__ void __launch_bounds__(kPwWarps * 32) paged_warp_kernel(const PagedPa
     };
     int64_t my_row = key_row();
     auto load_unit = [&](int stage) {              // issues the copies of ld_unit, then looks up the next
-        if (ld_unit < u_end) {
+        if (ld_more) {
             const uint32_t kdst = pipe + stage * 2 * TILE_B;
 #pragma unroll
             for (int i = 0; i < CH; ++i) {
@@ -265,7 +283,7 @@ __global__ void __launch_bounds__(kPwWarps * 32) paged_warp_kernel(const PagedPa
                 cp_async_16(kdst + pw_off<D>(r, c), p.K + off, n);
                 cp_async_16(kdst + TILE_B + pw_off<D>(r, c), p.V + off, n);
             }
-            ++ld_unit;
+            ++ld_j;
             my_row = key_row();
         }
         cp_async_commit();
@@ -274,12 +292,11 @@ __global__ void __launch_bounds__(kPwWarps * 32) paged_warp_kernel(const PagedPa
     for (int s = 0; s < kPwStages - 1; ++s) load_unit(s);
 
     // ---- arithmetic ------------------------------------------------------------------------
-    int tile = first_tile;
-    int stage = 0;
-    for (int u = u_begin; u < u_end; ++tile) {
+    int stage = 0, border = -1;
+    for (int tile = tile0; tile < tiles && p.start[tile] < u_end; ++tile) {
         const PagedTile t = p.tile[tile];
-        const int t_first = p.start[tile], t_next = p.start[tile + 1];
-        const int seg_end = min(u_end, t_next);
+        const int t_first = p.start[tile], t_units = (t.kv_end + kPwBN - 1) / kPwBN;
+        const int j0 = max(0, u_begin - t_first), j1 = min(t_units, u_end - t_first);
         // rows gid and gid + 8 of this lane: token (or -1) and the last key they see
         int head0 = 0, head1 = 0;
         const int i0 = gid < t.rows ? paged_row(p, t, gid, head0) : -1;
@@ -303,14 +320,14 @@ __global__ void __launch_bounds__(kPwWarps * 32) paged_warp_kernel(const PagedPa
         for (int j = 0; j < NT_O; ++j) { o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f; }
         float mx0 = -INFINITY, mx1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 
-        for (; u < seg_end; ++u) {
+        for (int j = j0; j < j1; ++j) {
             int fill = stage + kPwStages - 1;
             if (fill >= kPwStages) fill -= kPwStages;
             load_unit(fill);
             cp_async_wait<kPwStages - 1>();
             __syncwarp();
             const uint32_t kbase = pipe + stage * 2 * TILE_B, vbase = kbase + TILE_B;
-            const int kv0 = (u - t_first) * kPwBN;
+            const int kv0 = j * kPwBN;
             float s[NT_S][4];
 #pragma unroll
             for (int j = 0; j < NT_S; ++j) { s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f; }
@@ -394,7 +411,7 @@ __global__ void __launch_bounds__(kPwWarps * 32) paged_warp_kernel(const PagedPa
         l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
         l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
         l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-        if (t_first >= u_begin && t_next <= u_end) {         // the whole tile was this warp's
+        if (j1 - j0 == t_units) {                            // the whole tile was this warp's
             const float inv0 = l0 > 0.f ? 1.f / l0 : 0.f, inv1 = l1 > 0.f ? 1.f / l1 : 0.f;
             uint8_t* d0 = p.O + ((static_cast<int64_t>(t.tok0 + max(i0, 0)) * p.Hq + head0) * D + 2 * t4) * 2;
             uint8_t* d1 = p.O + ((static_cast<int64_t>(t.tok0 + max(i1, 0)) * p.Hq + head1) * D + 2 * t4) * 2;
@@ -406,6 +423,7 @@ __global__ void __launch_bounds__(kPwWarps * 32) paged_warp_kernel(const PagedPa
                     *reinterpret_cast<uint32_t*>(d1 + j * 16) = pack_half2<kBf16>(o[j][2] * inv1, o[j][3] * inv1);
             }
         } else {
+            if (j0 == 0) border = tile;
             const int64_t slot = (static_cast<int64_t>(worker) * 2 + (t_first > u_begin ? 1 : 0)) * kPwRows;
             float* d0 = p.part_o + (slot + gid) * D + 2 * t4;
             float* d1 = d0 + 8 * D;
@@ -422,79 +440,124 @@ __global__ void __launch_bounds__(kPwWarps * 32) paged_warp_kernel(const PagedPa
         }
     }
     cp_async_wait<0>();
+    if (lane == 0) p.border[worker] = border;
 }
 
 // ---- joining -----------------------------------------------------------------------------------
 
-// Block b < workers - 1 looks at the end of worker b's range: if a tile straddles it and this is the
-// tile's first such border, the block joins the tile's parts.  The other blocks write the rows that
-// no unit covers: routed out, without a visible key, and (clear_tail) behind the last sequence.
+// The first workers * row_groups blocks join the tiles that several workers shared: block (w, g) takes
+// the tile that starts in worker w's range and ends behind it, and every row_groups-th four rows of
+// it.  A warp joins a row of up to eight parts by itself, else the block's four warps share the row's
+// parts.  The other blocks write the rows that no unit covers, a token per warp: routed out,
+// without a visible key, and (clear_tail) behind the last sequence.
 template <int D, bool kBf16>
-__global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p, int join_blocks)
+__global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p, int row_groups)
 {
-    const int tid = threadIdx.x;
+    constexpr int C = D / 32;                                // columns of a lane
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    __shared__ float sh_o[4][D];
+    __shared__ float2 sh_ml[4];
+    paged_wait_previous();
+    const int join_blocks = p.workers * row_groups;
     if (static_cast<int>(blockIdx.x) < join_blocks) {
-        const int units = p.head->units, range = p.head->range;
-        const int64_t border = static_cast<int64_t>(blockIdx.x + 1) * range;
-        if (border >= units) return;
-        const int tile = paged_find_tile(p.start, p.head->tiles, static_cast<int>(border));
-        const int first = p.start[tile], end = p.start[tile + 1];
-        const int w0 = first / range, w1 = (end - 1) / range;
-        if (first == border || w0 != static_cast<int>(blockIdx.x)) return;
+        const int w0 = blockIdx.x / row_groups;
+        const int range = p.head->range, length = p.head->length;
+        if (static_cast<int64_t>(w0) * range >= length) return;
+        const int tile = p.border[w0];
+        if (tile < 0) return;
         const PagedTile t = p.tile[tile];
+        const int first = p.start[tile];
+        const int w1 = (first + (t.kv_end + p.unit_keys - 1) / p.unit_keys - 1) / range;
         const int slot0 = first > w0 * range ? 1 : 0;
-        constexpr int kRowsAtOnce = 128 / (D / 4);           // four columns per thread
-        const int c = (tid % (D / 4)) * 4;
-        for (int r = blockIdx.y * kRowsAtOnce + tid / (D / 4); r < t.rows; r += gridDim.y * kRowsAtOnce) {
+        const bool alone = w1 - w0 < 8;
+        const int step = alone ? 1 : 4;
+        const int r_step = row_groups * (alone ? 4 : 1);
+        const int r_first = (blockIdx.x - w0 * row_groups) * (alone ? 4 : 1) + (alone ? warp : 0);
+        for (int r = r_first; r < t.rows; r += r_step) {
             int head;
             const int i = paged_row(p, t, r, head);
             if (i < 0) continue;
-            float m = -INFINITY, l = 0.f;
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int w = w0; w <= w1; ++w) {
-                const int64_t slot = (static_cast<int64_t>(w) * 2 + (w == w0 ? slot0 : 0)) * p.tile_rows + r;
-                const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
-                const float4 x = *reinterpret_cast<const float4*>(p.part_o + slot * D + c);
-                if (ml.x == -INFINITY) continue;
-                const float top = fmaxf(m, ml.x);
-                const float a = m == -INFINITY ? 0.f : paged_exp2((m - top) * p.scale_log2);
-                const float b = paged_exp2((ml.x - top) * p.scale_log2);
-                l = l * a + ml.y * b;
-                acc.x = acc.x * a + x.x * b;
-                acc.y = acc.y * a + x.y * b;
-                acc.z = acc.z * a + x.z * b;
-                acc.w = acc.w * a + x.w * b;
-                m = top;
+            float m = -INFINITY, l = 0.f, acc[C];
+#pragma unroll
+            for (int c = 0; c < C; ++c) acc[c] = 0.f;
+            for (int w = w0 + (alone ? 0 : warp); w <= w1; w += 4 * step) {
+                // four parts in flight
+                float2 ml[4];
+                float x[4][C];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int v = w + k * step;
+                    ml[k] = make_float2(-INFINITY, 0.f);
+                    if (v <= w1) {
+                        const int64_t slot = (static_cast<int64_t>(v) * 2 + (v == w0 ? slot0 : 0)) * p.tile_rows + r;
+                        ml[k] = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
+                        const float* src = p.part_o + slot * D + lane * C;
+#pragma unroll
+                        for (int c = 0; c < C; c += 2) *reinterpret_cast<float2*>(&x[k][c]) = *reinterpret_cast<const float2*>(src + c);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    if (ml[k].x == -INFINITY) continue;
+                    const float top = fmaxf(m, ml[k].x);
+                    const float a = paged_exp2((m - top) * p.scale_log2), b = paged_exp2((ml[k].x - top) * p.scale_log2);
+                    l = l * a + ml[k].y * b;
+#pragma unroll
+                    for (int c = 0; c < C; ++c) acc[c] = acc[c] * a + x[k][c] * b;
+                    m = top;
+                }
+            }
+            if (!alone) {                                    // the same for the whole block
+#pragma unroll
+                for (int c = 0; c < C; ++c) sh_o[warp][lane * C + c] = acc[c];
+                if (lane == 0) sh_ml[warp] = make_float2(m, l);
+                __syncthreads();
+                if (warp == 0) {
+                    m = fmaxf(fmaxf(sh_ml[0].x, sh_ml[1].x), fmaxf(sh_ml[2].x, sh_ml[3].x));
+                    l = 0.f;
+#pragma unroll
+                    for (int c = 0; c < C; ++c) acc[c] = 0.f;
+                    for (int k = 0; k < 4; ++k) {
+                        if (sh_ml[k].x == -INFINITY) continue;
+                        const float b = paged_exp2((sh_ml[k].x - m) * p.scale_log2);
+                        l += sh_ml[k].y * b;
+#pragma unroll
+                        for (int c = 0; c < C; ++c) acc[c] += sh_o[k][lane * C + c] * b;
+                    }
+                }
+                __syncthreads();
+                if (warp != 0) continue;
             }
             const float inv = l > 0.f ? 1.f / l : 0.f;
-            uint2 out;
-            out.x = pack_half2<kBf16>(acc.x * inv, acc.y * inv);
-            out.y = pack_half2<kBf16>(acc.z * inv, acc.w * inv);
-            *reinterpret_cast<uint2*>(p.O + ((static_cast<int64_t>(t.tok0 + i) * p.Hq + head) * D + c) * 2) = out;
+            uint8_t* out = p.O + ((static_cast<int64_t>(t.tok0 + i) * p.Hq + head) * D + lane * C) * 2;
+#pragma unroll
+            for (int c = 0; c < C; c += 2)
+                *reinterpret_cast<uint32_t*>(out + c * 2) = pack_half2<kBf16>(acc[c] * inv, acc[c + 1] * inv);
         }
         return;
     }
-    if (blockIdx.y) return;
-    for (int t = blockIdx.x - join_blocks; t < p.N; t += gridDim.x - join_blocks) {
+    for (int t = (blockIdx.x - join_blocks) * 4 + warp; t < p.N; t += (gridDim.x - join_blocks) * 4) {
         const bool tail = p.S == 0 || t >= p.qstart[p.S];
+        if (tail && !p.clear_tail) continue;
         int seen = -1;                                       // last key the token sees
         if (!tail) {
-            int lo = 0, hi = p.S - 1;
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (p.qstart[mid] <= t) lo = mid;
-                else hi = mid - 1;
+            int lo = 0, hi = p.S;                            // last sequence that starts at or before t
+            while (hi - lo > 1) {
+                const int step = (hi - lo + 31) / 32;
+                const int at = lo + lane * step;
+                const bool ok = lane == 0 || (at < hi && p.qstart[at] <= t);
+                const int n = __popc(__ballot_sync(0xffffffffu, ok));
+                hi = min(hi, lo + n * step);
+                lo = lo + (n - 1) * step;
             }
             const int len = p.kv_lens[lo];
             seen = len <= 0 || len > static_cast<int64_t>(p.W) * p.page ? -1
                    : p.causal ? min(len - 1, len - p.qstart[lo + 1] + t) : len - 1;
         }
-        if (tail && !p.clear_tail) continue;
-        for (int x = tid; x < p.Hq * (D / 8); x += 128) {
+        if (seen >= 0 && !p.mask) continue;
+        for (int x = lane; x < p.Hq * (D / 8); x += 32) {
             const int head = x / (D / 8);
-            const bool dead = tail || seen < 0 ||
-                              (p.mask && p.mask[static_cast<int64_t>(t) * p.NG + head / p.hpg] == 0);
-            if (dead)
+            if (seen < 0 || p.mask[static_cast<int64_t>(t) * p.NG + head / p.hpg] == 0)
                 *reinterpret_cast<uint4*>(p.O + (static_cast<int64_t>(t) * p.Hq * D + x * 8) * 2) =
                     make_uint4(0, 0, 0, 0);
         }
@@ -506,8 +569,7 @@ static int launch_warp(const PagedParams& p, cudaStream_t s)
 {
     constexpr size_t smem = size_t(kPwWarps) * kPwStages * 2 * kPwBN * D * 2;
     DPK_CUDA(cudaFuncSetAttribute(paged_warp_kernel<D, kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    paged_warp_kernel<D, kBf16><<<p.workers / kPwWarps, kPwWarps * 32, smem, s>>>(p);
-    DPK_CUDA(cudaGetLastError());
+    DPK_CUDA(paged_launch(paged_warp_kernel<D, kBf16>, dim3(p.workers / kPwWarps), kPwWarps * 32, smem, s, p));
     return DPK_OK;
 }
 
@@ -520,22 +582,20 @@ int attn_paged_warp(const PagedParams& p, int D, int dtype, cudaStream_t s)
 template <int D, bool kBf16>
 static int launch_join(const PagedParams& p, cudaStream_t s)
 {
-    const int join = p.workers - 1;
-    int zero = p.N;
+    const int groups = p.tile_rows <= 16 ? 4 : 8;
+    int zero = (p.N + 3) / 4;
     const int cap = sm_count() * 16;
     if (zero > cap) zero = cap;
-    const int slices = p.tile_rows <= 16 ? 1 : 8;
-    paged_join_kernel<D, kBf16><<<dim3(join + zero, slices), 128, 0, s>>>(p, join);
-    DPK_CUDA(cudaGetLastError());
+    DPK_CUDA(paged_launch(paged_join_kernel<D, kBf16>, dim3(p.workers * groups + zero), 128, 0, s, p, groups));
     return DPK_OK;
 }
 
 // Which kernel, and how the work is cut, from what the host knows.
 struct PagedShape {
     bool tc;
-    int tile_rows, unit_keys, workers, min_range;
+    int tile_rows, unit_keys, tile_gap, workers, min_range;
     int64_t max_tiles;
-    size_t off_start, off_tile, off_first, off_rows, off_count, off_o, off_ml, bytes;
+    size_t off_start, off_tile, off_first, off_rows, off_count, off_border, off_o, off_ml, bytes;
 };
 
 static PagedShape paged_shape(int64_t N, int S, int Hq, int Hk, int D, int max_query_len, bool has_mask, int sms)
@@ -548,6 +608,7 @@ static PagedShape paged_shape(int64_t N, int S, int Hq, int Hk, int D, int max_q
     g.tile_rows = g.tc ? 128 : kPwRows;
     g.unit_keys = g.tc ? 64 : kPwBN;
     g.workers = g.tc ? 2 * sms : sms * kPwWarps;
+    g.tile_gap = g.tc ? 3 : 1;
     g.min_range = 2;
     g.max_tiles = int64_t(Hk) * ((N * rep) / g.tile_rows + S);
     size_t at = 16;
@@ -561,6 +622,7 @@ static PagedShape paged_shape(int64_t N, int S, int Hq, int Hk, int D, int max_q
     g.off_first = take(size_t(S) * Hk * 4);
     g.off_rows = take(g.tc && has_mask ? size_t(Hk) * N * rep * 4 : 0);
     g.off_count = take(g.tc && has_mask ? size_t(S) * Hk * 4 : 0);
+    g.off_border = take(size_t(g.workers) * 4);
     g.off_o = take(size_t(g.workers) * 2 * g.tile_rows * D * 4);
     g.off_ml = take(size_t(g.workers) * 2 * g.tile_rows * 8);
     g.bytes = at;
@@ -612,7 +674,7 @@ int dpk_attn_paged(const void* Q, const void* K, const void* V, const int32_t* p
     if (N == 0) return DPK_OK;
     const int sms = sm_count();
     const PagedShape g = paged_shape(N, S, Hq, Hk, D, max_query_len, mask != nullptr, sms);
-    DPK_REQUIRE(g.max_tiles * (int64_t(W) * page_size / g.unit_keys + 1) < (1ll << 31),
+    DPK_REQUIRE(g.max_tiles * (int64_t(W) * page_size / g.unit_keys + 1 + g.tile_gap) < (1ll << 31),
                 "too much work for one call: %lld tiles of up to %lld keys", (long long)g.max_tiles,
                 (long long)W * page_size);
     DPK_REQUIRE(int64_t(Hq) * N < (1ll << 31), "too many rows for one call");
@@ -643,21 +705,28 @@ int dpk_attn_paged(const void* Q, const void* K, const void* V, const int32_t* p
     p.first_tile = reinterpret_cast<int32_t*>(w + g.off_first);
     p.rows = g.tc && mask ? reinterpret_cast<int32_t*>(w + g.off_rows) : nullptr;
     p.row_count = g.tc && mask ? reinterpret_cast<int32_t*>(w + g.off_count) : nullptr;
+    p.border = reinterpret_cast<int32_t*>(w + g.off_border);
     p.part_o = reinterpret_cast<float*>(w + g.off_o);
     p.part_ml = reinterpret_cast<float*>(w + g.off_ml);
-    p.tile_rows = g.tile_rows; p.unit_keys = g.unit_keys;
+    p.tile_rows = g.tile_rows; p.unit_keys = g.unit_keys; p.tile_gap = g.tile_gap;
     p.workers = g.workers; p.min_range = g.min_range;
     p.max_tiles = static_cast<int>(g.max_tiles);
     p.status = device_status_ptr();
     if (!p.status) return fail(DPK_ERR_CUDA, "no status word on this device");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const int64_t items = static_cast<int64_t>(S) * Hk;
+    const int plan_threads = items <= 256 && g.max_tiles <= 512 ? 256 : kPlanThreads;
     if (p.rows && S > 0) {
         DPK_REQUIRE(Hk <= 65535, "grid too large");
-        paged_rows_kernel<<<dim3(S, Hk), max_query_len * p.rep > 512 ? 1024 : 128, 0, s>>>(p);
+        const int64_t per_thread = (static_cast<int64_t>(max_query_len) * p.rep + 15) / 16;
+        const int threads = per_thread >= 1024 ? 1024 : static_cast<int>((per_thread + 31) / 32 * 32);
+        paged_rows_kernel<<<dim3(S, Hk), threads, 0, s>>>(p);
+        DPK_CUDA(cudaGetLastError());
+        DPK_CUDA(paged_launch(paged_plan_kernel, dim3(1), plan_threads, 0, s, p));
+    } else {
+        paged_plan_kernel<<<1, plan_threads, 0, s>>>(p);
         DPK_CUDA(cudaGetLastError());
     }
-    paged_plan_kernel<<<1, kPlanThreads, 0, s>>>(p);
-    DPK_CUDA(cudaGetLastError());
     // without a page there is nothing to load: every length is 0, and the work list is empty
     if (P > 0) {
         const int rc = g.tc ? attn_paged_tc(p, D, dtype, s) : attn_paged_warp(p, D, dtype, s);

@@ -3,13 +3,14 @@
 //
 // The work is cut into TILES and UNITS.  A tile is up to `tile_rows` (new token, query head) rows of
 // one sequence and one KV head; a unit is `unit_keys` consecutive keys of a tile's visible range.
-// The units of all tiles form one line, and worker w (a warp or a CTA) takes units
-// [w * range, (w + 1) * range): sequences of very different lengths load the GPU evenly, a long
-// cache with few rows is split over many workers, and nothing depends on lengths the host does not
-// know.  A tile that one worker covers is finished there; of the others every worker leaves its
-// un-normalised sum, its row maxima and row sums in one of its two slots (slot 0 for the tile that
-// was begun by an earlier worker or starts with the range, slot 1 for the tile that starts later),
-// and the joining kernel adds them in worker order: the same bits on every run.
+// The units of all tiles form one line, with `tile_gap` empty places behind each tile for what a
+// tile costs beside its units, and worker w (a warp or a CTA) takes places [w * range, (w + 1) *
+// range): sequences of very different lengths load the GPU evenly, a long cache with few rows is
+// split over many workers, and nothing depends on lengths the host does not know.  A tile that one
+// worker covers is finished there; of the others every worker leaves its un-normalised sum, its row
+// maxima and row sums in one of its two slots (slot 0 for the tile that was begun by an earlier
+// worker or starts with the range, slot 1 for the tile that starts later), and the joining kernel
+// adds them in worker order: the same bits on every run.
 #pragma once
 
 #include "dpk_host.h"
@@ -28,8 +29,8 @@ struct PagedTile {
 
 struct PagedHead {          // written by the planning kernel
     int32_t tiles;          // tiles with work
-    int32_t units;          // units of all of them
-    int32_t range;          // units per worker
+    int32_t length;         // places of the line
+    int32_t range;          // places per worker
     int32_t pad;
 };
 
@@ -48,14 +49,15 @@ struct PagedParams {
     float scale_log2;
     // workspace
     PagedHead* head;
-    int32_t* start;         // [tiles + 1] first unit of each tile
+    int32_t* start;         // [tiles + 1] place of each tile's first unit
     PagedTile* tile;        // [tiles]
     int32_t* first_tile;    // [S * Hk + 1] running number of tiles before dropping empty ones
     int32_t* rows;          // [Hk][N * rep] active rows of each (sequence, KV head), or NULL: all rows
     int32_t* row_count;     // [S * Hk] with `rows`
+    int32_t* border;        // [workers] the tile that starts in the worker's range and ends behind it, or -1
     float* part_o;          // [workers][2][tile_rows][D]
     float* part_ml;         // [workers][2][tile_rows][2]
-    int tile_rows, unit_keys, workers, min_range, max_tiles;
+    int tile_rows, unit_keys, tile_gap, workers, min_range, max_tiles;
     int* status;
 };
 
@@ -70,20 +72,42 @@ __device__ __forceinline__ int paged_row(const PagedParams& p, const PagedTile& 
     return i;
 }
 
-// Last tile whose first unit is at or before `unit`; the whole warp searches, 32 probes a step.
-__device__ __forceinline__ int paged_find_tile(const int32_t* start, int tiles, int unit)
+// First tile with units at or behind `place`; the whole warp searches, 32 probes a step.
+__device__ __forceinline__ int paged_find_tile(const PagedParams& p, int tiles, int place)
 {
-    int lo = 0, hi = tiles;                         // answer in [lo, hi)
+    int lo = 0, hi = tiles;                         // the last tile that starts at or before `place`
     const int lane = threadIdx.x & 31;
     while (hi - lo > 1) {
         const int step = (hi - lo + 31) / 32;
         const int at = lo + lane * step;
-        const bool ok = at < hi && start[at] <= unit;
+        const bool ok = at < hi && p.start[at] <= place;
         const int n = __popc(__ballot_sync(0xffffffffu, ok));      // lane 0 always holds
         hi = min(hi, lo + n * step);
         lo = lo + (n - 1) * step;
     }
-    return lo;
+    return place < p.start[lo] + (p.tile[lo].kv_end + p.unit_keys - 1) / p.unit_keys ? lo : lo + 1;
+}
+
+// Kernels of one call follow each other without the gap between dependent launches: a kernel is
+// resident before its predecessor has ended, and waits here for the predecessor's writes.
+__device__ __forceinline__ void paged_wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void paged_let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <class... KArgs, class... Args>
+static cudaError_t paged_launch(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t s,
+                                Args... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
 __device__ __forceinline__ float paged_exp2(float x)

@@ -60,15 +60,21 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int units = p.head->units, range = p.head->range;
+    paged_wait_previous();
+    paged_let_next_start();
+    const int tiles = p.head->tiles, length = p.head->length, range = p.head->range;
     const int worker = blockIdx.x;
-    if (static_cast<int64_t>(worker) * range >= units) return;      // whole CTA: nothing allocated yet
+    if (static_cast<int64_t>(worker) * range >= length) return;     // whole CTA: nothing allocated yet
     if ((smem_u32(smem) & 1023u) != 0u) {
         if (threadIdx.x == 0) atomicCAS(p.status, 0, 1000 * DPK_KERNEL_ID + DPK_DEV_BAD_SMEM_BASE);
         return;
     }
-    const int u_begin = worker * range, u_end = min(units, u_begin + range);
-    const int tile0 = paged_find_tile(p.start, p.head->tiles, u_begin);
+    const int u_begin = worker * range, u_end = min(length, u_begin + range);
+    const int tile0 = paged_find_tile(p, tiles, u_begin);
+    if (tile0 >= tiles || p.start[tile0] >= u_end) {                // only places between tiles
+        if (threadIdx.x == 0) p.border[worker] = -1;
+        return;
+    }
 
     if (warp == 4 && lane == 0) {
         mbar_init(q_full, 128);
@@ -99,46 +105,59 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
         bool alive = true;
         int it = 0;                                     // units done, over all tiles
-        for (int tile = tile0, u = u_begin; alive && u < u_end; ++tile) {
-            const PagedTile t = p.tile[tile];
-            const int t_first = p.start[tile], t_next = p.start[tile + 1];
-            const int seg_end = min(u_end, t_next);
-            // Q rows into the swizzled K-major layout (8 lanes per 128 bytes, 16 rows per pass).
-            // The scores of the last tile's last unit were waited for: nothing reads the old Q.
-            {
-                const int chunk = threadIdx.x & 7, rsub = threadIdx.x >> 3;
-                for (int r = rsub; r < kPtBM; r += 16) {
-                    int head = 0;
-                    const int i = r < t.rows ? paged_row(p, t, r, head) : -1;
-                    const uint8_t* src = p.Q;
-                    if (i >= 0) src += (static_cast<int64_t>(t.tok0 + i) * p.q_ts + static_cast<int64_t>(head) * D) * 2;
+        int border = -1;
+        // Q rows into the swizzled K-major layout (8 lanes per 128 bytes, 16 rows per pass), and what
+        // this thread has to know about its own row
+        auto load_q = [&](const PagedTile& t, int& tok, int& head) {
+            const int chunk = threadIdx.x & 7, rsub = threadIdx.x >> 3;
+            for (int r = rsub; r < kPtBM; r += 16) {
+                int h = 0;
+                const int i = r < t.rows ? paged_row(p, t, r, h) : -1;
+                const uint8_t* src = p.Q;
+                if (i >= 0) src += (static_cast<int64_t>(t.tok0 + i) * p.q_ts + static_cast<int64_t>(h) * D) * 2;
 #pragma unroll
-                    for (int kb = 0; kb < KBQ; ++kb)
-                        cp_async_16(smem_u32(sQ) + kb * (kPtBM * 128) + r * 128 + ((chunk ^ (r & 7)) << 4),
-                                    src + kb * 128 + chunk * 16, i >= 0 ? 16u : 0u);
-                }
-                cp_async_commit();
+                for (int kb = 0; kb < KBQ; ++kb)
+                    cp_async_16(smem_u32(sQ) + kb * (kPtBM * 128) + r * 128 + ((chunk ^ (r & 7)) << 4),
+                                src + kb * 128 + chunk * 16, i >= 0 ? 16u : 0u);
             }
-            int head = 0, head0 = 0;
-            const int tok = row < t.rows ? paged_row(p, t, row, head) : -1;
+            cp_async_commit();
+            head = 0;
+            tok = row < t.rows ? paged_row(p, t, row, head) : -1;
+        };
+        auto q_ready = [&]() {
+            cp_async_wait<0>();
+            fence_proxy_async_smem();
+            mbar_arrive(q_full);
+        };
+        PagedTile t = p.tile[tile0], nt = t;
+        int tok, head, ntok = -1, nhead = 0;
+        load_q(t, tok, head);
+        q_ready();
+        bool more = true;
+        for (int tile = tile0; alive && more; ++tile) {
+            const int t_first = p.start[tile], t_units = (t.kv_end + kPtBN - 1) / kPtBN;
+            const int j0 = max(0, u_begin - t_first), j1 = min(t_units, u_end - t_first);
+            more = tile + 1 < tiles && p.start[tile + 1] < u_end;
+            if (more) nt = p.tile[tile + 1];
+            int head0 = 0;
             const int tok_first = paged_row(p, t, 0, head0);
             const int lim = tok < 0 ? -1 : p.causal ? min(t.kv_len - 1, t.pos0 + tok) : t.kv_len - 1;
             // the fewest keys that a row of the tile sees (rows are in token order)
             const int lim_first = p.causal ? min(t.kv_len - 1, t.pos0 + tok_first) : t.kv_len - 1;
             const bool idle = warp * 32 >= t.rows;      // none of this warp's rows exists
-            cp_async_wait<0>();
-            fence_proxy_async_smem();
-            mbar_arrive(q_full);
 
             float m_ref = -INFINITY, l_sum = 0.f;
             const int seg_it = it;
-            for (; u < seg_end; ++u, ++it) {
+            for (int j = j0; j < j1; ++j, ++it) {
                 const int sb = it & 1;
                 const uint32_t ph = (it >> 1) & 1;
                 const bool got = mbar_wait(&s_full[sb], ph, abort_flag, p.status, DPK_DEV_TIMEOUT_TMEM_FULL);
                 if (!__all_sync(0xffffffffu, got)) { alive = false; break; }
                 tc_fence_after_sync();
-                const int kv0 = (u - t_first) * kPtBN;
+                // the scores of the tile's last unit are there, so nothing reads Q any more: the next
+                // tile's rows come in while this unit is worked on
+                if (j == j1 - 1 && more) load_q(nt, ntok, nhead);
+                const int kv0 = j * kPtBN;
                 if (kv0 + kPtBN > t.kv_end && t.kv_end % box_rows != 0) {
                     // rows of V behind the last visible key that arrived with their box
                     const bool ok = mbar_wait(&v_full[sb], ph, abort_flag, p.status, DPK_DEV_TIMEOUT_FULL);
@@ -238,6 +257,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 mbar_arrive(&p_full[sb]);
             }
             if (!alive) break;
+            if (more) q_ready();
 
             // ---- epilogue: the row, finished or as this worker's part ----------------------
             const int pb = (it - 1) & 1;
@@ -246,7 +266,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             if (!__all_sync(0xffffffffu, ok)) break;
             tc_fence_after_sync();
             if (!idle) {
-                const bool whole = t_first >= u_begin && t_next <= u_end;
+                const bool whole = j1 - j0 == t_units;
                 const float inv = l_sum > 0.f ? 1.f / l_sum : 0.f;
                 const int64_t slot = (static_cast<int64_t>(worker) * 2 + (t_first > u_begin ? 1 : 0)) * kPtBM + row;
                 uint8_t* out = p.O + (static_cast<int64_t>(t.tok0 + max(tok, 0)) * p.Hq + head) * (D * 2);
@@ -276,30 +296,38 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 }
                 if (!whole && tok >= 0) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(m_ref, l_sum);
             }
+            if (j0 == 0 && j1 < t_units) border = tile;
             tc_fence_before_sync();     // the next tile's first P V overwrites O after these reads
+            t = nt;
+            tok = ntok;
+            head = nhead;
         }
+        cp_async_wait<0>();
+        if (threadIdx.x == 0) p.border[worker] = border;
     } else if (warp == 4) {
         // =================== producer: lane b loads box b of every unit ===================
         const int boxes = kPtBN / box_rows;
         const uint32_t box_bytes = box_rows * 128;
-        int tile = tile0, u = u_begin;
-        PagedTile t = p.tile[tile];
-        int t_first = p.start[tile], t_next = p.start[tile + 1];
+        int tile = tile0 - 1, j_next = 0, j_end = 0;
+        bool have = true;                               // there is a next unit
+        PagedTile t;
         // page and row of this lane's box of the next unit; a page outside the map reads as zeros
         int next_page = p.P, next_row = 0, next_col = 0;
         auto look_up = [&]() {
             next_page = p.P;
             next_row = 0;
-            if (u >= u_end) return;
-            if (u >= t_next) {
+            if (j_next >= j_end) {
                 ++tile;
+                const int first = tile < tiles ? p.start[tile] : length;
+                have = first < u_end;
+                if (!have) return;
                 t = p.tile[tile];
-                t_first = t_next;
-                t_next = p.start[tile + 1];
+                j_next = max(0, u_begin - first);
+                j_end = min((t.kv_end + kPtBN - 1) / kPtBN, u_end - first);
             }
             next_col = t.kvh * D;
-            const int key = (u - t_first) * kPtBN + lane * box_rows;
-            ++u;
+            const int key = j_next * kPtBN + lane * box_rows;
+            ++j_next;
             if (lane >= boxes || key >= t.kv_end) return;
             const int w = key / p.page;
             const int id = p.table[t.seq * p.table_stride + w];
@@ -311,13 +339,13 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             next_row = key - w * p.page;
         };
         look_up();
-        const int n = u_end - u_begin;
         int v_page = 0, v_row = 0, v_col = 0;           // the unit whose V is loaded next
-        bool live = true;
+        bool live = true, last = false;
         // K runs one unit ahead of V: it is needed one softmax earlier and released earlier
-        for (int j = 0; live && j <= n; ++j) {
+        for (int j = 0; live && !last; ++j) {
             const int k_page = next_page, k_row = next_row, k_col = next_col;
-            if (j < n) {
+            last = !have;
+            if (!last) {
                 look_up();
                 const int s = j & 1;
                 live = mbar_wait(&k_empty[s], ((j >> 1) & 1) ^ 1, abort_flag, p.status, DPK_DEV_TIMEOUT_EMPTY);
@@ -357,9 +385,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             const uint32_t idesc_o = umma_idesc_f16(kBf16 ? 1 : 0, kPtBM, D) | (1u << 16);   // B is MN-major
             bool ok = true;
             int it = 0, seg = 0;
-            for (int tile = tile0, u = u_begin; ok && u < u_end; ++tile, ++seg) {
-                const int len = min(u_end, p.start[tile + 1]) - u;
-                u += len;
+            for (int tile = tile0; ok && tile < tiles && p.start[tile] < u_end; ++tile, ++seg) {
+                const int first = p.start[tile];
+                const int len = min((p.tile[tile].kv_end + kPtBN - 1) / kPtBN, u_end - first) - max(0, u_begin - first);
                 ok = mbar_wait(q_full, seg & 1, abort_flag, p.status, DPK_DEV_TIMEOUT_FULL);
                 auto issue_s = [&](int i) -> bool {
                     const int s = i & 1;
@@ -422,8 +450,7 @@ static int launch_tc(const PagedParams& p, cudaStream_t s)
     if (rc) return rc;
     constexpr int smem = PtSmem<D>::kTotal;
     DPK_CUDA(cudaFuncSetAttribute(paged_tc_kernel<D, kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    paged_tc_kernel<D, kBf16><<<p.workers, kPtThreads, smem, s>>>(tmK, tmV, p, box);
-    DPK_CUDA(cudaGetLastError());
+    DPK_CUDA(paged_launch(paged_tc_kernel<D, kBf16>, dim3(p.workers), kPtThreads, smem, s, tmK, tmV, p, box));
     return DPK_OK;
 }
 

@@ -26,30 +26,32 @@ namespace dpk {
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanItems = 4096;        // (sequence, KV head) pairs whose tile numbers fit shared memory
 
-__device__ __forceinline__ int plan_scan(int v, int* sh, int& total)
+// Sum over the block's threads, for two values at once; `sh` holds 32 pairs.  Every thread gets the
+// totals and the sums of the threads before it.
+__device__ __forceinline__ int2 plan_scan(int2 v, int2* sh, int2& total)
 {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    int x = v;
+    int2 x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
+        const int y = __shfl_up_sync(0xffffffffu, x.x, o), z = __shfl_up_sync(0xffffffffu, x.y, o);
+        if (lane >= o) { x.x += y; x.y += z; }
     }
-    __syncthreads();
+    __syncthreads();                       // the previous use of sh is over
     if (lane == 31) sh[warp] = x;
     __syncthreads();
-    if (warp == 0) {
-        int w = lane < warps ? sh[lane] : 0;
+    int2 w = lane < warps ? sh[lane] : make_int2(0, 0);
+    int2 before = make_int2(0, 0);
+    total = make_int2(0, 0);
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, w, o);
-            if (lane >= o) w += y;
-        }
-        sh[lane] = w;
+    for (int k = 0; k < 32; ++k) {
+        if (k >= warps) break;
+        const int y = __shfl_sync(0xffffffffu, w.x, k), z = __shfl_sync(0xffffffffu, w.y, k);
+        if (k < warp) { before.x += y; before.y += z; }
+        total.x += y;
+        total.y += z;
     }
-    __syncthreads();
-    total = sh[warps - 1];
-    return x - v + (warp ? sh[warp - 1] : 0);
+    return make_int2(x.x - v.x + before.x, x.y - v.y + before.y);
 }
 
 // New tokens of sequence s, 0 where query_start does not make sense.
@@ -69,7 +71,7 @@ __device__ __forceinline__ int plan_new(const PagedParams& p, int s, int& tok0)
 // none of them is spent on a routed-out (token, head).  A thread looks at 16 rows in a row.
 __global__ void __launch_bounds__(1024) paged_rows_kernel(const PagedParams p)
 {
-    __shared__ int sh[33];
+    __shared__ int2 sh[32];
     paged_let_next_start();
     const int s = blockIdx.x, kvh = blockIdx.y;
     int tok0;
@@ -91,23 +93,20 @@ __global__ void __launch_bounds__(1024) paged_rows_kernel(const PagedParams p)
                 }
             }
         }
-        int t;
-        int at = carry + plan_scan(__popc(on), sh, t);
+        int2 t;
+        int at = carry + plan_scan(make_int2(__popc(on), 0), sh, t).x;
         for (; on; on &= on - 1) out[at++] = x + __ffs(on) - 1;
-        carry += t;
+        carry += t.x;
     }
     if (threadIdx.x == 0) p.row_count[s * p.Hk + kvh] = carry;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedParams p)
+// The whole block cuts the work: `tile`, `start` [tiles + 1] and `first` [S * Hk] may be shared memory.
+__device__ __forceinline__ void plan_work(const PagedParams& p, PagedTile* tile, int32_t* start, int* first,
+                                          int2* sh, int& tiles_out, int& length_out)
 {
-    __shared__ int sh[33];
-    __shared__ int sh_first[kPlanItems];
     const int tid = threadIdx.x, threads = blockDim.x;
     const int items = p.S * p.Hk;
-    int* first = items <= kPlanItems ? sh_first : p.first_tile;
-    paged_let_next_start();
-    if (p.rows) paged_wait_previous();
     // 1. tiles of every (sequence, KV head)
     int carry = 0;
     for (int x0 = 0; x0 < items; x0 += threads) {
@@ -115,14 +114,13 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedPar
         int n = 0;
         if (x < items) {
             int tok0;
-            const int s = x / p.Hk;
-            const int rows = p.rows ? p.row_count[x] : plan_new(p, s, tok0) * p.rep;
+            const int rows = p.rows ? p.row_count[x] : plan_new(p, x / p.Hk, tok0) * p.rep;
             n = (rows + p.tile_rows - 1) / p.tile_rows;
         }
-        int t;
-        const int at = plan_scan(n, sh, t);
-        if (x < items) first[x] = carry + at;
-        carry += t;
+        int2 t;
+        const int2 at = plan_scan(make_int2(n, 0), sh, t);
+        if (x < items) first[x] = carry + at.x;
+        carry += t.x;
     }
     const int tiles = min(carry, p.max_tiles);
     __syncthreads();
@@ -152,35 +150,49 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedPar
             }
             pt.pos0 = pt.kv_len - fresh;
             pt.kv_end = pt.kv_len;
-            int any = 1;
-            if (p.causal || (p.mask && !p.rows)) {
-                any = 0;
-                int last = -1, head;
-                if (p.rows || !p.mask) {
-                    last = paged_row(p, pt, pt.rows - 1, head);
-                } else {
-                    for (int r = pt.rows - 1; r >= 0 && last < 0; --r) last = paged_row(p, pt, r, head);
-                }
-                any = last >= 0;
-                if (p.causal) pt.kv_end = min(pt.kv_len, pt.pos0 + last + 1);
+            int last = 0, head;
+            if (p.rows || !p.mask) {
+                if (p.causal) last = paged_row(p, pt, pt.rows - 1, head);
+            } else {                                 // the last row that is not routed out
+                last = -1;
+                for (int r = pt.rows - 1; r >= 0 && last < 0; --r) last = paged_row(p, pt, r, head);
             }
-            if (any && pt.kv_end > 0) n = (pt.kv_end + p.unit_keys - 1) / p.unit_keys;
+            if (p.causal) pt.kv_end = min(pt.kv_len, pt.pos0 + last + 1);
+            if (last >= 0 && pt.kv_end > 0) n = paged_units(p, pt);
         }
-        int total, some;
-        const int slot = kept + plan_scan(n > 0, sh, some);
-        const int place = length + plan_scan(n > 0 ? n + p.tile_gap : 0, sh, total);
+        int2 total;
+        const int2 at = plan_scan(make_int2(n > 0, n > 0 ? n + p.tile_gap : 0), sh, total);
         if (n > 0) {
-            p.tile[slot] = pt;
-            p.start[slot] = place;
+            tile[kept + at.x] = pt;
+            start[kept + at.x] = length + at.y;
         }
-        kept += some;
-        length += total;
+        kept += total.x;
+        length += total.y;
     }
-    if (tid == 0) {
-        p.start[kept] = length;
-        p.head->tiles = kept;
+    if (tid == 0) start[kept] = length;
+    __syncthreads();
+    tiles_out = kept;
+    length_out = length;
+}
+
+__device__ __forceinline__ int plan_range(const PagedParams& p, int length)
+{
+    return max((length + p.workers - 1) / p.workers, p.min_range);
+}
+
+__global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedParams p)
+{
+    __shared__ int2 sh[32];
+    __shared__ int sh_first[kPlanItems];
+    paged_let_next_start();
+    if (p.rows) paged_wait_previous();
+    int tiles, length;
+    plan_work(p, p.tile, p.start, static_cast<int64_t>(p.S) * p.Hk <= kPlanItems ? sh_first : p.first_tile, sh, tiles,
+              length);
+    if (threadIdx.x == 0) {
+        p.head->tiles = tiles;
         p.head->length = length;
-        p.head->range = max((length + p.workers - 1) / p.workers, p.min_range);
+        p.head->range = plan_range(p, length);
     }
 }
 
@@ -226,7 +238,13 @@ __device__ __forceinline__ uint32_t pw_off(int r, int c)
     return static_cast<uint32_t>(r * (D * 2) + ((c ^ (r & 7)) << 4));
 }
 
-template <int D, bool kBf16>
+// Up to kPwTiles tiles (a decode step of 16 sequences with 8 KV heads) the attention kernel makes the work
+// list itself, every CTA for its own use in shared memory behind the rings: that saves a launch of a
+// kernel that takes as long as a small step's attention (8 tiles: 22 us a call instead of 27).  A
+// CTA of 128 threads takes longer over a long list than the launch does (512 tiles: 262 us instead of 258).
+constexpr int kPwTiles = 144;
+
+template <int D, bool kBf16, bool kPlanHere>
 __global__ void __launch_bounds__(kPwWarps * 32) paged_warp_kernel(const PagedParams p)
 {
     constexpr int CH = D / 8, KS = D / 16, NT_S = kPwBN / 8, NT_O = D / 8;
@@ -237,13 +255,29 @@ __global__ void __launch_bounds__(kPwWarps * 32) paged_warp_kernel(const PagedPa
     const int gid = lane >> 2, t4 = lane & 3;
     const uint32_t pipe = smem_u32(smem + warp * WARP_B);
 
-    paged_wait_previous();
+    int tiles, length, range;
+    PagedTile* tile_of = p.tile;
+    int32_t* start = p.start;
     paged_let_next_start();
-    const int tiles = p.head->tiles, length = p.head->length, range = p.head->range;
+    if constexpr (kPlanHere) {
+        __shared__ int2 sh[32];
+        tile_of = reinterpret_cast<PagedTile*>(smem + kPwWarps * WARP_B);
+        start = reinterpret_cast<int32_t*>(tile_of + kPwTiles);
+        plan_work(p, tile_of, start, start + kPwTiles + 1, sh, tiles, length);
+        range = plan_range(p, length);
+    } else {
+        paged_wait_previous();
+        tiles = p.head->tiles;
+        length = p.head->length;
+        range = p.head->range;
+    }
     const int worker = blockIdx.x * kPwWarps + warp;
-    if (static_cast<int64_t>(worker) * range >= length) return;
+    if (static_cast<int64_t>(worker) * range >= length) {
+        if (lane == 0 && worker < p.workers) p.border[worker].last_worker = -1;
+        return;
+    }
     const int u_begin = worker * range, u_end = min(length, u_begin + range);
-    const int tile0 = paged_find_tile(p, tiles, u_begin);
+    const int tile0 = paged_find_tile(p, tile_of, start, tiles, u_begin);
 
     // ---- loader: two units ahead of the arithmetic, across the ends of tiles -----------------
     int ld_tile = tile0 - 1, ld_j = 0, ld_n = 0;   // ld_j: the unit of ld_tile to be loaded next
@@ -253,10 +287,10 @@ __global__ void __launch_bounds__(kPwWarps * 32) paged_warp_kernel(const PagedPa
     auto key_row = [&]() -> int64_t {
         if (ld_j >= ld_n) {
             ++ld_tile;
-            const int first = ld_tile < tiles ? p.start[ld_tile] : length;
+            const int first = ld_tile < tiles ? start[ld_tile] : length;
             ld_more = first < u_end;
             if (!ld_more) return -1;
-            lt = p.tile[ld_tile];
+            lt = tile_of[ld_tile];
             ld_j = max(0, u_begin - first);
             ld_n = min((lt.kv_end + kPwBN - 1) / kPwBN, u_end - first);
         }
@@ -292,10 +326,10 @@ __global__ void __launch_bounds__(kPwWarps * 32) paged_warp_kernel(const PagedPa
     for (int s = 0; s < kPwStages - 1; ++s) load_unit(s);
 
     // ---- arithmetic ------------------------------------------------------------------------
-    int stage = 0, border = -1;
-    for (int tile = tile0; tile < tiles && p.start[tile] < u_end; ++tile) {
-        const PagedTile t = p.tile[tile];
-        const int t_first = p.start[tile], t_units = (t.kv_end + kPwBN - 1) / kPwBN;
+    int stage = 0, border = -1;         // border: the tile that ends behind this warp's range
+    for (int tile = tile0; tile < tiles && start[tile] < u_end; ++tile) {
+        const PagedTile t = tile_of[tile];
+        const int t_first = start[tile], t_units = (t.kv_end + kPwBN - 1) / kPwBN;
         const int j0 = max(0, u_begin - t_first), j1 = min(t_units, u_end - t_first);
         // rows gid and gid + 8 of this lane: token (or -1) and the last key they see
         int head0 = 0, head1 = 0;
@@ -440,99 +474,130 @@ __global__ void __launch_bounds__(kPwWarps * 32) paged_warp_kernel(const PagedPa
         }
     }
     cp_async_wait<0>();
-    if (lane == 0) p.border[worker] = border;
+    if (lane == 0) paged_write_border(p, tile_of, start, worker, border, u_begin, range);
 }
 
 // ---- joining -----------------------------------------------------------------------------------
 
-// The first workers * row_groups blocks join the tiles that several workers shared: block (w, g) takes
-// the tile that starts in worker w's range and ends behind it, and every row_groups-th four rows of
-// it.  A warp joins a row of up to eight parts by itself, else the block's four warps share the row's
-// parts.  The other blocks write the rows that no unit covers, a token per warp: routed out,
-// without a visible key, and (clear_tail) behind the last sequence.
-template <int D, bool kBf16>
-__global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p, int row_groups)
+// The first join_blocks = workers * row_groups blocks join the tiles that several workers shared: block
+// (w, g) takes a share of the rows of the tile that starts in worker w's range and ends behind it.
+// Where that are up to eight parts a warp joins kRows rows by itself, their loads in flight
+// together; else the block's four warps share the parts of each row.  The other blocks write the
+// rows that no unit covers, a token per warp: routed out, without a visible key, and (clear_tail)
+// behind the last sequence.
+struct JoinRow {
+    float m, l;
+};
+
+template <int C>
+__device__ __forceinline__ void join_add(JoinRow& s, float (&acc)[C], const float2& ml, const float (&x)[C], float scale_log2)
+{
+    if (ml.x == -INFINITY) return;
+    const float top = fmaxf(s.m, ml.x);
+    const float a = paged_exp2((s.m - top) * scale_log2), b = paged_exp2((ml.x - top) * scale_log2);
+    s.l = s.l * a + ml.y * b;
+#pragma unroll
+    for (int c = 0; c < C; ++c) acc[c] = acc[c] * a + x[c] * b;
+    s.m = top;
+}
+
+template <int C>
+__device__ __forceinline__ void join_load(const PagedParams& p, int64_t slot, int D, int lane, float2& ml, float (&x)[C])
+{
+    ml = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
+    const float* src = p.part_o + slot * D + lane * C;
+#pragma unroll
+    for (int c = 0; c < C; c += 2) *reinterpret_cast<float2*>(&x[c]) = *reinterpret_cast<const float2*>(src + c);
+}
+
+template <int D, bool kBf16, int kRows>
+__global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p, int row_groups, int join_blocks)
 {
     constexpr int C = D / 32;                                // columns of a lane
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     __shared__ float sh_o[4][D];
     __shared__ float2 sh_ml[4];
     paged_wait_previous();
-    const int join_blocks = p.workers * row_groups;
     if (static_cast<int>(blockIdx.x) < join_blocks) {
-        const int w0 = blockIdx.x / row_groups;
-        const int range = p.head->range, length = p.head->length;
-        if (static_cast<int64_t>(w0) * range >= length) return;
-        const int tile = p.border[w0];
-        if (tile < 0) return;
-        const PagedTile t = p.tile[tile];
-        const int first = p.start[tile];
-        const int w1 = (first + (t.kv_end + p.unit_keys - 1) / p.unit_keys - 1) / range;
-        const int slot0 = first > w0 * range ? 1 : 0;
-        const bool alone = w1 - w0 < 8;
-        const int step = alone ? 1 : 4;
-        const int r_step = row_groups * (alone ? 4 : 1);
-        const int r_first = (blockIdx.x - w0 * row_groups) * (alone ? 4 : 1) + (alone ? warp : 0);
-        for (int r = r_first; r < t.rows; r += r_step) {
-            int head;
-            const int i = paged_row(p, t, r, head);
-            if (i < 0) continue;
-            float m = -INFINITY, l = 0.f, acc[C];
-#pragma unroll
-            for (int c = 0; c < C; ++c) acc[c] = 0.f;
-            for (int w = w0 + (alone ? 0 : warp); w <= w1; w += 4 * step) {
-                // four parts in flight
-                float2 ml[4];
-                float x[4][C];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int v = w + k * step;
-                    ml[k] = make_float2(-INFINITY, 0.f);
-                    if (v <= w1) {
-                        const int64_t slot = (static_cast<int64_t>(v) * 2 + (v == w0 ? slot0 : 0)) * p.tile_rows + r;
-                        ml[k] = *reinterpret_cast<const float2*>(p.part_ml + slot * 2);
-                        const float* src = p.part_o + slot * D + lane * C;
-#pragma unroll
-                        for (int c = 0; c < C; c += 2) *reinterpret_cast<float2*>(&x[k][c]) = *reinterpret_cast<const float2*>(src + c);
-                    }
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    if (ml[k].x == -INFINITY) continue;
-                    const float top = fmaxf(m, ml[k].x);
-                    const float a = paged_exp2((m - top) * p.scale_log2), b = paged_exp2((ml[k].x - top) * p.scale_log2);
-                    l = l * a + ml[k].y * b;
-#pragma unroll
-                    for (int c = 0; c < C; ++c) acc[c] = acc[c] * a + x[k][c] * b;
-                    m = top;
-                }
-            }
-            if (!alone) {                                    // the same for the whole block
-#pragma unroll
-                for (int c = 0; c < C; ++c) sh_o[warp][lane * C + c] = acc[c];
-                if (lane == 0) sh_ml[warp] = make_float2(m, l);
-                __syncthreads();
-                if (warp == 0) {
-                    m = fmaxf(fmaxf(sh_ml[0].x, sh_ml[1].x), fmaxf(sh_ml[2].x, sh_ml[3].x));
-                    l = 0.f;
-#pragma unroll
-                    for (int c = 0; c < C; ++c) acc[c] = 0.f;
-                    for (int k = 0; k < 4; ++k) {
-                        if (sh_ml[k].x == -INFINITY) continue;
-                        const float b = paged_exp2((sh_ml[k].x - m) * p.scale_log2);
-                        l += sh_ml[k].y * b;
-#pragma unroll
-                        for (int c = 0; c < C; ++c) acc[c] += sh_o[k][lane * C + c] * b;
-                    }
-                }
-                __syncthreads();
-                if (warp != 0) continue;
-            }
-            const float inv = l > 0.f ? 1.f / l : 0.f;
+        const int w0 = blockIdx.x / row_groups, group = blockIdx.x - w0 * row_groups;
+        const PagedBorder border = p.border[w0];
+        const PagedTile& t = border.tile;
+        const int w1 = border.last_worker, slot0 = border.slot;
+        if (w1 < 0) return;
+        auto slot_of = [&](int w, int r) { return (static_cast<int64_t>(w) * 2 + (w == w0 ? slot0 : 0)) * p.tile_rows + r; };
+        auto store = [&](int i, int head, const JoinRow& s, const float (&acc)[C]) {
+            const float inv = s.l > 0.f ? 1.f / s.l : 0.f;
             uint8_t* out = p.O + ((static_cast<int64_t>(t.tok0 + i) * p.Hq + head) * D + lane * C) * 2;
 #pragma unroll
             for (int c = 0; c < C; c += 2)
                 *reinterpret_cast<uint32_t*>(out + c * 2) = pack_half2<kBf16>(acc[c] * inv, acc[c + 1] * inv);
+        };
+        if (w1 - w0 < 8) {
+            for (int r = (group * 4 + warp) * kRows; r < t.rows; r += row_groups * 4 * kRows) {
+                int i[kRows], head[kRows];
+                JoinRow s[kRows];
+                float acc[kRows][C];
+#pragma unroll
+                for (int k = 0; k < kRows; ++k) {
+                    i[k] = r + k < t.rows ? paged_row(p, t, r + k, head[k]) : -1;
+                    s[k] = {-INFINITY, 0.f};
+#pragma unroll
+                    for (int c = 0; c < C; ++c) acc[k][c] = 0.f;
+                }
+                for (int w = w0; w <= w1; w += 2) {
+                    float2 ml[2][kRows];
+                    float x[2][kRows][C];
+#pragma unroll
+                    for (int v = 0; v < 2; ++v)
+#pragma unroll
+                        for (int k = 0; k < kRows; ++k) {
+                            ml[v][k] = make_float2(-INFINITY, 0.f);
+                            if (i[k] >= 0 && w + v <= w1) join_load<C>(p, slot_of(w + v, r + k), D, lane, ml[v][k], x[v][k]);
+                        }
+#pragma unroll
+                    for (int v = 0; v < 2; ++v)
+#pragma unroll
+                        for (int k = 0; k < kRows; ++k) join_add<C>(s[k], acc[k], ml[v][k], x[v][k], p.scale_log2);
+                }
+#pragma unroll
+                for (int k = 0; k < kRows; ++k)
+                    if (i[k] >= 0) store(i[k], head[k], s[k], acc[k]);
+            }
+            return;
+        }
+        for (int r = group; r < t.rows; r += row_groups) {
+            int head;
+            const int i = paged_row(p, t, r, head);
+            if (i < 0) continue;
+            JoinRow s = {-INFINITY, 0.f};
+            float acc[C];
+#pragma unroll
+            for (int c = 0; c < C; ++c) acc[c] = 0.f;
+            for (int w = w0 + warp; w <= w1; w += 16) {
+                float2 ml[4];
+                float x[4][C];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    ml[k] = make_float2(-INFINITY, 0.f);
+                    if (w + 4 * k <= w1) join_load<C>(p, slot_of(w + 4 * k, r), D, lane, ml[k], x[k]);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) join_add<C>(s, acc, ml[k], x[k], p.scale_log2);
+            }
+#pragma unroll
+            for (int c = 0; c < C; ++c) sh_o[warp][lane * C + c] = acc[c];
+            if (lane == 0) sh_ml[warp] = make_float2(s.m, s.l);
+            __syncthreads();
+            if (warp == 0) {
+                for (int k = 1; k < 4; ++k) {
+                    float x[C];
+#pragma unroll
+                    for (int c = 0; c < C; ++c) x[c] = sh_o[k][lane * C + c];
+                    join_add<C>(s, acc, sh_ml[k], x, p.scale_log2);
+                }
+                store(i, head, s, acc);
+            }
+            __syncthreads();
         }
         return;
     }
@@ -565,28 +630,43 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p, in
 }
 
 template <int D, bool kBf16>
-static int launch_warp(const PagedParams& p, cudaStream_t s)
+static int launch_warp(const PagedParams& p, int used, bool plan_here, cudaStream_t s)
 {
-    constexpr size_t smem = size_t(kPwWarps) * kPwStages * 2 * kPwBN * D * 2;
-    DPK_CUDA(cudaFuncSetAttribute(paged_warp_kernel<D, kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    DPK_CUDA(paged_launch(paged_warp_kernel<D, kBf16>, dim3(p.workers / kPwWarps), kPwWarps * 32, smem, s, p));
+    constexpr int rings = kPwWarps * kPwStages * 2 * kPwBN * D * 2;
+    constexpr int lists = kPwTiles * int(sizeof(PagedTile)) + (2 * kPwTiles + 1) * 4;
+    const dim3 grid((used + kPwWarps - 1) / kPwWarps);
+    if (plan_here) {
+        DPK_CUDA(cudaFuncSetAttribute(paged_warp_kernel<D, kBf16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      rings + lists));
+        paged_warp_kernel<D, kBf16, true><<<grid, kPwWarps * 32, rings + lists, s>>>(p);
+        DPK_CUDA(cudaGetLastError());
+    } else {
+        DPK_CUDA(cudaFuncSetAttribute(paged_warp_kernel<D, kBf16, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                      rings));
+        DPK_CUDA(paged_launch(paged_warp_kernel<D, kBf16, false>, grid, kPwWarps * 32, rings, s, p));
+    }
     return DPK_OK;
 }
 
-int attn_paged_warp(const PagedParams& p, int D, int dtype, cudaStream_t s)
+int attn_paged_warp(const PagedParams& p, int D, int dtype, int used, bool plan_here, cudaStream_t s)
 {
-    if (D == 64) return dtype == DPK_BF16 ? launch_warp<64, true>(p, s) : launch_warp<64, false>(p, s);
-    return dtype == DPK_BF16 ? launch_warp<128, true>(p, s) : launch_warp<128, false>(p, s);
+    if (D == 64)
+        return dtype == DPK_BF16 ? launch_warp<64, true>(p, used, plan_here, s)
+                                 : launch_warp<64, false>(p, used, plan_here, s);
+    return dtype == DPK_BF16 ? launch_warp<128, true>(p, used, plan_here, s)
+                             : launch_warp<128, false>(p, used, plan_here, s);
 }
 
 template <int D, bool kBf16>
-static int launch_join(const PagedParams& p, cudaStream_t s)
+static int launch_join(const PagedParams& p, int used, cudaStream_t s)
 {
-    const int groups = p.tile_rows <= 16 ? 4 : 8;
     int zero = (p.N + 3) / 4;
-    const int cap = sm_count() * 16;
+    const int cap = sm_count() * 4;
     if (zero > cap) zero = cap;
-    DPK_CUDA(paged_launch(paged_join_kernel<D, kBf16>, dim3(p.workers * groups + zero), 128, 0, s, p, groups));
+    if (p.tile_rows <= 16)
+        DPK_CUDA(paged_launch(paged_join_kernel<D, kBf16, 1>, dim3(used * 4 + zero), 128, 0, s, p, 4, used * 4));
+    else
+        DPK_CUDA(paged_launch(paged_join_kernel<D, kBf16, 2>, dim3(used * 4 + zero), 128, 0, s, p, 4, used * 4));
     return DPK_OK;
 }
 
@@ -595,6 +675,7 @@ struct PagedShape {
     bool tc;
     int tile_rows, unit_keys, tile_gap, workers, min_range;
     int64_t max_tiles;
+    bool plan_here;
     size_t off_start, off_tile, off_first, off_rows, off_count, off_border, off_o, off_ml, bytes;
 };
 
@@ -611,6 +692,7 @@ static PagedShape paged_shape(int64_t N, int S, int Hq, int Hk, int D, int max_q
     g.tile_gap = g.tc ? 3 : 1;
     g.min_range = 2;
     g.max_tiles = int64_t(Hk) * ((N * rep) / g.tile_rows + S);
+    g.plan_here = !g.tc && g.max_tiles <= kPwTiles && int64_t(S) * Hk <= kPwTiles;
     size_t at = 16;
     auto take = [&](size_t bytes) {
         const size_t here = at;
@@ -622,7 +704,7 @@ static PagedShape paged_shape(int64_t N, int S, int Hq, int Hk, int D, int max_q
     g.off_first = take(size_t(S) * Hk * 4);
     g.off_rows = take(g.tc && has_mask ? size_t(Hk) * N * rep * 4 : 0);
     g.off_count = take(g.tc && has_mask ? size_t(S) * Hk * 4 : 0);
-    g.off_border = take(size_t(g.workers) * 4);
+    g.off_border = take(size_t(g.workers) * sizeof(PagedBorder));
     g.off_o = take(size_t(g.workers) * 2 * g.tile_rows * D * 4);
     g.off_ml = take(size_t(g.workers) * 2 * g.tile_rows * 8);
     g.bytes = at;
@@ -674,9 +756,9 @@ int dpk_attn_paged(const void* Q, const void* K, const void* V, const int32_t* p
     if (N == 0) return DPK_OK;
     const int sms = sm_count();
     const PagedShape g = paged_shape(N, S, Hq, Hk, D, max_query_len, mask != nullptr, sms);
-    DPK_REQUIRE(g.max_tiles * (int64_t(W) * page_size / g.unit_keys + 1 + g.tile_gap) < (1ll << 31),
-                "too much work for one call: %lld tiles of up to %lld keys", (long long)g.max_tiles,
-                (long long)W * page_size);
+    const int64_t most = g.max_tiles * ((int64_t(W) * page_size + g.unit_keys - 1) / g.unit_keys + g.tile_gap);
+    DPK_REQUIRE(most < (1ll << 31), "too much work for one call: %lld tiles of up to %lld keys",
+                (long long)g.max_tiles, (long long)W * page_size);
     DPK_REQUIRE(int64_t(Hq) * N < (1ll << 31), "too many rows for one call");
     DPK_REQUIRE(workspace && workspace_bytes >= g.bytes, "workspace of %zu bytes needed, %zu given", g.bytes,
                 workspace_bytes);
@@ -691,7 +773,9 @@ int dpk_attn_paged(const void* Q, const void* K, const void* V, const int32_t* p
     p.qstart = query_start;
     p.mask = mask;
     p.q_ts = q_ts; p.page_stride = ps; p.token_stride = kv_ts; p.table_stride = ts;
-    p.N = static_cast<int>(N); p.S = S; p.W = W; p.P = P; p.page = page_size;
+    p.N = static_cast<int>(N); p.S = S; p.P = P;
+    p.W = P > 0 ? W : 0;                       // without a page no length can be right
+    p.page = page_size;
     p.Hq = Hq; p.Hk = Hk; p.NG = mask ? NG : 1;
     p.rep = Hq / Hk;
     p.hpg = Hq / p.NG;
@@ -705,7 +789,7 @@ int dpk_attn_paged(const void* Q, const void* K, const void* V, const int32_t* p
     p.first_tile = reinterpret_cast<int32_t*>(w + g.off_first);
     p.rows = g.tc && mask ? reinterpret_cast<int32_t*>(w + g.off_rows) : nullptr;
     p.row_count = g.tc && mask ? reinterpret_cast<int32_t*>(w + g.off_count) : nullptr;
-    p.border = reinterpret_cast<int32_t*>(w + g.off_border);
+    p.border = reinterpret_cast<PagedBorder*>(w + g.off_border);
     p.part_o = reinterpret_cast<float*>(w + g.off_o);
     p.part_ml = reinterpret_cast<float*>(w + g.off_ml);
     p.tile_rows = g.tile_rows; p.unit_keys = g.unit_keys; p.tile_gap = g.tile_gap;
@@ -714,8 +798,11 @@ int dpk_attn_paged(const void* Q, const void* K, const void* V, const int32_t* p
     p.status = device_status_ptr();
     if (!p.status) return fail(DPK_ERR_CUDA, "no status word on this device");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const int64_t items = static_cast<int64_t>(S) * Hk;
-    const int plan_threads = items <= 256 && g.max_tiles <= 512 ? 256 : kPlanThreads;
+    // workers that can get work at all, as far as the host knows
+    int64_t used = (most + g.min_range - 1) / g.min_range;
+    if (used > g.workers) used = g.workers;
+    if (used < 1) used = 1;
+    const int plan_threads = int64_t(S) * Hk <= 256 && g.max_tiles <= 512 ? 256 : kPlanThreads;
     if (p.rows && S > 0) {
         DPK_REQUIRE(Hk <= 65535, "grid too large");
         const int64_t per_thread = (static_cast<int64_t>(max_query_len) * p.rep + 15) / 16;
@@ -723,17 +810,15 @@ int dpk_attn_paged(const void* Q, const void* K, const void* V, const int32_t* p
         paged_rows_kernel<<<dim3(S, Hk), threads, 0, s>>>(p);
         DPK_CUDA(cudaGetLastError());
         DPK_CUDA(paged_launch(paged_plan_kernel, dim3(1), plan_threads, 0, s, p));
-    } else {
+    } else if (!g.plan_here) {
         paged_plan_kernel<<<1, plan_threads, 0, s>>>(p);
         DPK_CUDA(cudaGetLastError());
     }
-    // without a page there is nothing to load: every length is 0, and the work list is empty
-    if (P > 0) {
-        const int rc = g.tc ? attn_paged_tc(p, D, dtype, s) : attn_paged_warp(p, D, dtype, s);
-        if (rc) return rc;
-    }
-    if (D == 64) return dtype == DPK_BF16 ? launch_join<64, true>(p, s) : launch_join<64, false>(p, s);
-    return dtype == DPK_BF16 ? launch_join<128, true>(p, s) : launch_join<128, false>(p, s);
+    const int rc = g.tc ? attn_paged_tc(p, D, dtype, static_cast<int>(used), s)
+                        : attn_paged_warp(p, D, dtype, static_cast<int>(used), g.plan_here, s);
+    if (rc) return rc;
+    if (D == 64) return dtype == DPK_BF16 ? launch_join<64, true>(p, (int)used, s) : launch_join<64, false>(p, (int)used, s);
+    return dtype == DPK_BF16 ? launch_join<128, true>(p, (int)used, s) : launch_join<128, false>(p, (int)used, s);
 }
 
 }  // extern "C"

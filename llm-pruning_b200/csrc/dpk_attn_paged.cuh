@@ -34,6 +34,14 @@ struct PagedHead {          // written by the planning kernel
     int32_t pad;
 };
 
+// Left by each worker for the joining kernel: the tile that starts in its range and ends behind it.
+struct PagedBorder {
+    PagedTile tile;
+    int32_t last_worker;    // the worker that ends the tile; -1: there is no such tile
+    int32_t slot;           // where this worker left its part; later ones use slot 0
+    int32_t pad[2];
+};
+
 struct PagedParams {
     const uint8_t* Q;       // [N, Hq, D]
     const uint8_t* K;       // [P, page, Hk, D]
@@ -54,7 +62,7 @@ struct PagedParams {
     int32_t* first_tile;    // [S * Hk + 1] running number of tiles before dropping empty ones
     int32_t* rows;          // [Hk][N * rep] active rows of each (sequence, KV head), or NULL: all rows
     int32_t* row_count;     // [S * Hk] with `rows`
-    int32_t* border;        // [workers] the tile that starts in the worker's range and ends behind it, or -1
+    PagedBorder* border;    // [workers]
     float* part_o;          // [workers][2][tile_rows][D]
     float* part_ml;         // [workers][2][tile_rows][2]
     int tile_rows, unit_keys, tile_gap, workers, min_range, max_tiles;
@@ -72,20 +80,39 @@ __device__ __forceinline__ int paged_row(const PagedParams& p, const PagedTile& 
     return i;
 }
 
+__device__ __forceinline__ int paged_units(const PagedParams& p, const PagedTile& t)
+{
+    return (t.kv_end + p.unit_keys - 1) / p.unit_keys;
+}
+
 // First tile with units at or behind `place`; the whole warp searches, 32 probes a step.
-__device__ __forceinline__ int paged_find_tile(const PagedParams& p, int tiles, int place)
+__device__ __forceinline__ int paged_find_tile(const PagedParams& p, const PagedTile* tile, const int32_t* start,
+                                               int tiles, int place)
 {
     int lo = 0, hi = tiles;                         // the last tile that starts at or before `place`
     const int lane = threadIdx.x & 31;
     while (hi - lo > 1) {
         const int step = (hi - lo + 31) / 32;
         const int at = lo + lane * step;
-        const bool ok = at < hi && p.start[at] <= place;
+        const bool ok = at < hi && start[at] <= place;
         const int n = __popc(__ballot_sync(0xffffffffu, ok));      // lane 0 always holds
         hi = min(hi, lo + n * step);
         lo = lo + (n - 1) * step;
     }
-    return place < p.start[lo] + (p.tile[lo].kv_end + p.unit_keys - 1) / p.unit_keys ? lo : lo + 1;
+    return place < start[lo] + paged_units(p, tile[lo]) ? lo : lo + 1;
+}
+
+__device__ __forceinline__ void paged_write_border(const PagedParams& p, const PagedTile* tile, const int32_t* start,
+                                                   int worker, int border, int u_begin, int range)
+{
+    PagedBorder b;
+    b.last_worker = -1;
+    if (border >= 0) {
+        b.tile = tile[border];
+        b.last_worker = (start[border] + paged_units(p, b.tile) - 1) / range;
+        b.slot = start[border] > u_begin ? 1 : 0;
+    }
+    p.border[worker] = b;
 }
 
 // Kernels of one call follow each other without the gap between dependent launches: a kernel is
@@ -117,7 +144,7 @@ __device__ __forceinline__ float paged_exp2(float x)
     return y;
 }
 
-int attn_paged_warp(const PagedParams& p, int D, int dtype, cudaStream_t s);
-int attn_paged_tc(const PagedParams& p, int D, int dtype, cudaStream_t s);
+// `used`: workers that can get work
+int attn_paged_tc(const PagedParams& p, int D, int dtype, int used, cudaStream_t s);
 
 }  // namespace dpk

@@ -64,15 +64,18 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     paged_let_next_start();
     const int tiles = p.head->tiles, length = p.head->length, range = p.head->range;
     const int worker = blockIdx.x;
-    if (static_cast<int64_t>(worker) * range >= length) return;     // whole CTA: nothing allocated yet
+    if (static_cast<int64_t>(worker) * range >= length) {           // whole CTA: nothing allocated yet
+        if (threadIdx.x == 0) p.border[worker].last_worker = -1;
+        return;
+    }
     if ((smem_u32(smem) & 1023u) != 0u) {
         if (threadIdx.x == 0) atomicCAS(p.status, 0, 1000 * DPK_KERNEL_ID + DPK_DEV_BAD_SMEM_BASE);
         return;
     }
     const int u_begin = worker * range, u_end = min(length, u_begin + range);
-    const int tile0 = paged_find_tile(p, tiles, u_begin);
+    const int tile0 = paged_find_tile(p, p.tile, p.start, tiles, u_begin);
     if (tile0 >= tiles || p.start[tile0] >= u_end) {                // only places between tiles
-        if (threadIdx.x == 0) p.border[worker] = -1;
+        if (threadIdx.x == 0) p.border[worker].last_worker = -1;
         return;
     }
 
@@ -106,23 +109,24 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         bool alive = true;
         int it = 0;                                     // units done, over all tiles
         int border = -1;
-        // Q rows into the swizzled K-major layout (8 lanes per 128 bytes, 16 rows per pass), and what
-        // this thread has to know about its own row
+        // Q rows into the swizzled K-major layout: every warp its own 32 rows (8 lanes per 128 bytes, four
+        // rows per pass; the rows' places in Q are looked up once, by the lane that owns the row)
         auto load_q = [&](const PagedTile& t, int& tok, int& head) {
-            const int chunk = threadIdx.x & 7, rsub = threadIdx.x >> 3;
-            for (int r = rsub; r < kPtBM; r += 16) {
-                int h = 0;
-                const int i = r < t.rows ? paged_row(p, t, r, h) : -1;
-                const uint8_t* src = p.Q;
-                if (i >= 0) src += (static_cast<int64_t>(t.tok0 + i) * p.q_ts + static_cast<int64_t>(h) * D) * 2;
+            head = 0;
+            tok = row < t.rows ? paged_row(p, t, row, head) : -1;
+            const int64_t mine = tok < 0 ? -1 : (static_cast<int64_t>(t.tok0 + tok) * p.q_ts + static_cast<int64_t>(head) * D) * 2;
+            const int chunk = lane & 7;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int sub = (lane >> 3) + 4 * k, r = warp * 32 + sub;
+                const int64_t at = __shfl_sync(0xffffffffu, mine, sub);
+                const uint8_t* src = p.Q + (at < 0 ? 0 : at);
 #pragma unroll
                 for (int kb = 0; kb < KBQ; ++kb)
                     cp_async_16(smem_u32(sQ) + kb * (kPtBM * 128) + r * 128 + ((chunk ^ (r & 7)) << 4),
-                                src + kb * 128 + chunk * 16, i >= 0 ? 16u : 0u);
+                                src + kb * 128 + chunk * 16, at >= 0 ? 16u : 0u);
             }
             cp_async_commit();
-            head = 0;
-            tok = row < t.rows ? paged_row(p, t, row, head) : -1;
         };
         auto q_ready = [&]() {
             cp_async_wait<0>();
@@ -130,20 +134,20 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             mbar_arrive(q_full);
         };
         PagedTile t = p.tile[tile0], nt = t;
+        int t_first = p.start[tile0];
         int tok, head, ntok = -1, nhead = 0;
         load_q(t, tok, head);
         q_ready();
         bool more = true;
         for (int tile = tile0; alive && more; ++tile) {
-            const int t_first = p.start[tile], t_units = (t.kv_end + kPtBN - 1) / kPtBN;
+            const int t_units = (t.kv_end + kPtBN - 1) / kPtBN;
             const int j0 = max(0, u_begin - t_first), j1 = min(t_units, u_end - t_first);
-            more = tile + 1 < tiles && p.start[tile + 1] < u_end;
+            const int n_first = p.start[tile + 1];           // what the next tile needs, long before
+            more = tile + 1 < tiles && n_first < u_end;
             if (more) nt = p.tile[tile + 1];
-            int head0 = 0;
-            const int tok_first = paged_row(p, t, 0, head0);
             const int lim = tok < 0 ? -1 : p.causal ? min(t.kv_len - 1, t.pos0 + tok) : t.kv_len - 1;
-            // the fewest keys that a row of the tile sees (rows are in token order)
-            const int lim_first = p.causal ? min(t.kv_len - 1, t.pos0 + tok_first) : t.kv_len - 1;
+            // the fewest keys that a row of the warp sees: its first row's (rows are in token order)
+            const int lim_first = __shfl_sync(0xffffffffu, lim, 0);
             const bool idle = warp * 32 >= t.rows;      // none of this warp's rows exists
 
             float m_ref = -INFINITY, l_sum = 0.f;
@@ -299,18 +303,20 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             if (j0 == 0 && j1 < t_units) border = tile;
             tc_fence_before_sync();     // the next tile's first P V overwrites O after these reads
             t = nt;
+            t_first = n_first;
             tok = ntok;
             head = nhead;
         }
         cp_async_wait<0>();
-        if (threadIdx.x == 0) p.border[worker] = border;
+        if (threadIdx.x == 0) paged_write_border(p, p.tile, p.start, worker, border, u_begin, range);
     } else if (warp == 4) {
         // =================== producer: lane b loads box b of every unit ===================
         const int boxes = kPtBN / box_rows;
         const uint32_t box_bytes = box_rows * 128;
         int tile = tile0 - 1, j_next = 0, j_end = 0;
         bool have = true;                               // there is a next unit
-        PagedTile t;
+        PagedTile t, nt = p.tile[tile0];
+        int n_first = p.start[tile0];
         // page and row of this lane's box of the next unit; a page outside the map reads as zeros
         int next_page = p.P, next_row = 0, next_col = 0;
         auto look_up = [&]() {
@@ -318,12 +324,13 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             next_row = 0;
             if (j_next >= j_end) {
                 ++tile;
-                const int first = tile < tiles ? p.start[tile] : length;
-                have = first < u_end;
+                have = tile < tiles && n_first < u_end;
                 if (!have) return;
-                t = p.tile[tile];
-                j_next = max(0, u_begin - first);
-                j_end = min((t.kv_end + kPtBN - 1) / kPtBN, u_end - first);
+                t = nt;
+                j_next = max(0, u_begin - n_first);
+                j_end = min((t.kv_end + kPtBN - 1) / kPtBN, u_end - n_first);
+                n_first = p.start[tile + 1];            // long before it is needed
+                if (tile + 1 < tiles) nt = p.tile[tile + 1];
             }
             next_col = t.kvh * D;
             const int key = j_next * kPtBN + lane * box_rows;
@@ -385,9 +392,11 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             const uint32_t idesc_o = umma_idesc_f16(kBf16 ? 1 : 0, kPtBM, D) | (1u << 16);   // B is MN-major
             bool ok = true;
             int it = 0, seg = 0;
-            for (int tile = tile0; ok && tile < tiles && p.start[tile] < u_end; ++tile, ++seg) {
-                const int first = p.start[tile];
-                const int len = min((p.tile[tile].kv_end + kPtBN - 1) / kPtBN, u_end - first) - max(0, u_begin - first);
+            int n_first = p.start[tile0], n_end = p.tile[tile0].kv_end;
+            for (int tile = tile0; ok && tile < tiles && n_first < u_end; ++tile, ++seg) {
+                const int len = min((n_end + kPtBN - 1) / kPtBN, u_end - n_first) - max(0, u_begin - n_first);
+                n_first = p.start[tile + 1];            // long before it is needed
+                if (tile + 1 < tiles) n_end = p.tile[tile + 1].kv_end;
                 ok = mbar_wait(q_full, seg & 1, abort_flag, p.status, DPK_DEV_TIMEOUT_FULL);
                 auto issue_s = [&](int i) -> bool {
                     const int s = i & 1;
@@ -438,7 +447,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
 }
 
 template <int D, bool kBf16>
-static int launch_tc(const PagedParams& p, cudaStream_t s)
+static int launch_tc(const PagedParams& p, int used, cudaStream_t s)
 {
     int box = 64;                                       // gcd(page, 64): page is a multiple of 8
     while (p.page % box) box >>= 1;
@@ -450,14 +459,14 @@ static int launch_tc(const PagedParams& p, cudaStream_t s)
     if (rc) return rc;
     constexpr int smem = PtSmem<D>::kTotal;
     DPK_CUDA(cudaFuncSetAttribute(paged_tc_kernel<D, kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    DPK_CUDA(paged_launch(paged_tc_kernel<D, kBf16>, dim3(p.workers), kPtThreads, smem, s, tmK, tmV, p, box));
+    DPK_CUDA(paged_launch(paged_tc_kernel<D, kBf16>, dim3(used), kPtThreads, smem, s, tmK, tmV, p, box));
     return DPK_OK;
 }
 
-int attn_paged_tc(const PagedParams& p, int D, int dtype, cudaStream_t s)
+int attn_paged_tc(const PagedParams& p, int D, int dtype, int used, cudaStream_t s)
 {
-    if (D == 64) return dtype == DPK_BF16 ? launch_tc<64, true>(p, s) : launch_tc<64, false>(p, s);
-    return dtype == DPK_BF16 ? launch_tc<128, true>(p, s) : launch_tc<128, false>(p, s);
+    if (D == 64) return dtype == DPK_BF16 ? launch_tc<64, true>(p, used, s) : launch_tc<64, false>(p, used, s);
+    return dtype == DPK_BF16 ? launch_tc<128, true>(p, used, s) : launch_tc<128, false>(p, used, s);
 }
 
 }  // namespace dpk

@@ -31,21 +31,34 @@ def _code(t: torch.Tensor) -> int:
     return code
 
 
-def _on_gpu(*tensors: Optional[torch.Tensor]) -> torch.device:
-    dev = tensors[0].device
+def _on_gpu(*tensors: Optional[torch.Tensor]) -> int:
+    """Index of the one CUDA device that holds all of them."""
+    dev = tensors[0].get_device()
+    if dev < 0:
+        raise ValueError("dpk_b200 operators run on CUDA tensors only (no CPU fallback)")
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise ValueError("dpk_b200 operators run on CUDA tensors only (no CPU fallback)")
-        if t.device != dev:
+        if t is not None and t.get_device() != dev:
+            if t.get_device() < 0:
+                raise ValueError("dpk_b200 operators run on CUDA tensors only (no CPU fallback)")
             raise ValueError("all tensors must be on the same device")
     return dev
 
 
+def _call(dev: int, entry, *args) -> None:
+    """One C entry point on the current stream of device ``dev``; entering the device is skipped where
+    it is the current one already (it costs as much as a launch)."""
+    if torch.cuda.current_device() == dev:
+        rc = entry(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = entry(*args, _raw_stream(dev))
+    if rc:
+        N.check(rc)
+
+
 def _ints(t: torch.Tensor, shape: tuple, name: str) -> torch.Tensor:
     """A contiguous int32 tensor of ``shape``."""
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape {list(shape)}, got "
                          f"{t.dtype} {list(t.shape)}")
     return t
@@ -83,6 +96,8 @@ def _token_rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     """``t [N,heads,D]`` with the heads of a token back to back: the tensor (copied only if it does
     not fit) and its token stride in elements."""
     n, heads, D = t.shape
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t, heads * D
     ts = t.stride(0) if n > 1 else heads * D
     if not ((D == 1 or t.stride(2) == 1) and (heads == 1 or t.stride(1) == D) and ts >= heads * D
             and ts % 8 == 0 and t.data_ptr() % 16 == 0):
@@ -91,8 +106,10 @@ def _token_rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     return t, ts
 
 
-def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+if _raw_stream is None:                 # a torch build without CUDA, or without this shortcut
+    def _raw_stream(dev: int) -> int:
+        return torch.cuda.current_stream(dev).cuda_stream
 
 
 def attention_paged(Q: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tensor,
@@ -141,7 +158,7 @@ def attention_paged(Q: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tenso
     Qc, q_ts = _token_rows(Q)
     clear = 0
     if O is None:
-        O = torch.empty((n, Hq, D), dtype=Q.dtype, device=dev)
+        O = Q.new_empty((n, Hq, D))
         clear = 1
     elif O.shape != Q.shape or O.dtype != Q.dtype or not O.is_contiguous():
         raise ValueError("O must be contiguous with the shape and dtype of Q")
@@ -150,18 +167,16 @@ def attention_paged(Q: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tenso
         raise ValueError("max_query_len must be at least 1")
     lib = N.load()
     nbytes = lib.dpk_attn_paged_workspace_bytes(n, S, Hq, Hk, D, most, 0 if m8 is None else 1)
-    with torch.cuda.device(dev):
-        ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-        N.check(lib.dpk_attn_paged(
-            Qc.data_ptr(), K_pages.data_ptr(), V_pages.data_ptr(), page_table.data_ptr(),
-            kv_lens.data_ptr(), query_start.data_ptr(), None if m8 is None else m8.data_ptr(),
-            O.data_ptr(), n, S, W, P, page, Hq, Hk, D, NG, D ** -0.5 if scale is None else float(scale),
-            1 if is_causal else 0, code, max(most, 1), clear, q_ts, ps, ts, tstride, ws.data_ptr(), nbytes,
-            _stream()))
+    ws = page_table.new_empty((nbytes + 3) // 4)
+    _call(dev, lib.dpk_attn_paged,
+          Qc.data_ptr(), K_pages.data_ptr(), V_pages.data_ptr(), page_table.data_ptr(), kv_lens.data_ptr(),
+          query_start.data_ptr(), None if m8 is None else m8.data_ptr(), O.data_ptr(), n, S, W, P, page, Hq,
+          Hk, D, NG, D ** -0.5 if scale is None else float(scale), 1 if is_causal else 0, code,
+          most if most > 1 else 1, clear, q_ts, ps, ts, tstride, ws.data_ptr(), nbytes)
     return O, {}
 
 
-def _rope(q, k, v, positions, inv_freq, sections, axis_map, interleaved, attention_scale, q_out, cache):
+def _rope(dev, q, k, v, positions, inv_freq, sections, axis_map, interleaved, attention_scale, q_out, cache):
     code = _code(q)
     if k.dtype != q.dtype or (v is not None and v.dtype != q.dtype):
         raise ValueError("q, k and v must share one dtype")
@@ -204,7 +219,7 @@ def _rope(q, k, v, positions, inv_freq, sections, axis_map, interleaved, attenti
             kc, vc = k.contiguous(), v.contiguous()
             kv_ts = Hk * D
     if q_out is None:
-        q_out = torch.empty((n, Hq, D), dtype=q.dtype, device=q.device)
+        q_out = q.new_empty((n, Hq, D))
         qo_ts = Hq * D
     else:
         if q_out.shape != q.shape or q_out.dtype != q.dtype:
@@ -214,7 +229,7 @@ def _rope(q, k, v, positions, inv_freq, sections, axis_map, interleaved, attenti
             raise ValueError("q_out: the heads of a token must be contiguous, 16-byte aligned")
     k_out = None
     if cache is None:
-        k_out = torch.empty((n, Hk, D), dtype=q.dtype, device=q.device)
+        k_out = q.new_empty((n, Hk, D))
         tail = (None, None, 0, 0, None, 0, None, None, n, 0, 0, 0, 0)
     else:
         k_pages, v_pages, page_table, kv_lens, query_start = cache
@@ -228,13 +243,12 @@ def _rope(q, k, v, positions, inv_freq, sections, axis_map, interleaved, attenti
         _ints(query_start, (S + 1,), "query_start")
         tail = (k_pages.data_ptr(), v_pages.data_ptr(), ps, ts, page_table.data_ptr(), tstride,
                 kv_lens.data_ptr(), query_start.data_ptr(), n, S, W, P, page)
-    with torch.cuda.device(q.device):
-        N.check(N.load().dpk_rope_append_paged(
-            qc.data_ptr(), kc.data_ptr(), None if vc is None else vc.data_ptr(), q_out.data_ptr(),
-            None if k_out is None else k_out.data_ptr(), q_ts, kv_ts, qo_ts, positions.data_ptr(),
-            axis_stride, 1 if positions.dtype == torch.int64 else 0, inv_freq.data_ptr(),
-            None if axis_map is None else axis_map.data_ptr(), secs, axes, rotary,
-            1 if interleaved else 0, float(attention_scale), *tail, Hq, Hk, D, code, _stream()))
+    _call(dev, N.load().dpk_rope_append_paged,
+          qc.data_ptr(), kc.data_ptr(), None if vc is None else vc.data_ptr(), q_out.data_ptr(),
+          None if k_out is None else k_out.data_ptr(), q_ts, kv_ts, qo_ts, positions.data_ptr(), axis_stride,
+          1 if positions.dtype is torch.int64 else 0, inv_freq.data_ptr(),
+          None if axis_map is None else axis_map.data_ptr(), secs, axes, rotary, 1 if interleaved else 0,
+          float(attention_scale), *tail, Hq, Hk, D, code)
     return q_out, k_out
 
 
@@ -257,8 +271,8 @@ def rope_append_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positio
     and sin.  A token's place in the cache is its place in the sequence (the last tokens of
     ``kv_lens[s]``), whatever its rotary positions.  Counterpart of :func:`rope_append`; computed
     from positions, so far ones keep their exact angle."""
-    _on_gpu(q, k, v, positions, inv_freq, K_pages, V_pages, page_table, kv_lens, query_start, axis_map, q_out)
-    return _rope(q, k, v, positions, inv_freq, sections, axis_map, interleaved, attention_scale, q_out,
+    dev = _on_gpu(q, k, v, positions, inv_freq, K_pages, V_pages, page_table, kv_lens, query_start, axis_map, q_out)
+    return _rope(dev, q, k, v, positions, inv_freq, sections, axis_map, interleaved, attention_scale, q_out,
                  (K_pages, V_pages, page_table, kv_lens, query_start))[0]
 
 
@@ -266,8 +280,8 @@ def rope_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_fre
               sections: Optional[Sequence[int]] = None, axis_map: Optional[torch.Tensor] = None,
               interleaved: bool = False, attention_scale: float = 1.0):
     """The rotation of :func:`rope_append_paged` without a cache: ``(rotated q, rotated k)``."""
-    _on_gpu(q, k, positions, inv_freq, axis_map)
-    return _rope(q, k, None, positions, inv_freq, sections, axis_map, interleaved, attention_scale, None, None)
+    dev = _on_gpu(q, k, positions, inv_freq, axis_map)
+    return _rope(dev, q, k, None, positions, inv_freq, sections, axis_map, interleaved, attention_scale, None, None)
 
 
 # ---------------------------------------------------------------------------------------- pages
@@ -299,9 +313,9 @@ def _pools(k_pages, v_pages):
     return (k_pages.data_ptr(), v_pages.data_ptr(), L, ls, ps, row), P, page
 
 
-def _workspace(S: int, P: int, n: int, dev):
+def _workspace(S: int, P: int, n: int, like: torch.Tensor):
     nbytes = N.load().dpk_page_workspace_bytes(S, P, n)
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev), nbytes
+    return like.new_empty((nbytes + 3) // 4), nbytes
 
 
 def _vector(t: torch.Tensor, name: str, n: Optional[int] = None) -> int:
@@ -324,11 +338,9 @@ def page_extend(K_pages: torch.Tensor, V_pages: torch.Tensor, page_table: torch.
     if P != st[6]:
         raise ValueError(f"ref_counts has {st[6]} entries, the pools have {P} pages")
     _vector(add, "add", st[4])
-    granted = torch.empty(st[4], dtype=torch.bool, device=dev)
-    with torch.cuda.device(dev):
-        ws, nbytes = _workspace(st[4], 0, 0, dev)
-        N.check(N.load().dpk_page_extend(*st, page, add.data_ptr(), granted.data_ptr(), *pools,
-                                         ws.data_ptr(), nbytes, _stream()))
+    granted = add.new_empty(st[4], dtype=torch.bool)
+    ws, nbytes = _workspace(st[4], 0, 0, add)
+    _call(dev, N.load().dpk_page_extend, *st, page, add.data_ptr(), granted.data_ptr(), *pools, ws.data_ptr(), nbytes)
     return granted
 
 
@@ -341,11 +353,10 @@ def page_fork(page_table: torch.Tensor, kv_lens: torch.Tensor, ref_counts: torch
     st = _state(page_table, kv_lens, ref_counts)
     n = _vector(parents, "parents")
     _vector(children, "children", n)
-    done = torch.empty(n, dtype=torch.bool, device=dev)
-    with torch.cuda.device(dev):
-        ws, nbytes = _workspace(0, 0, n, dev)
-        N.check(N.load().dpk_page_fork(*st, int(page_size), parents.data_ptr(), children.data_ptr(), n,
-                                       done.data_ptr(), ws.data_ptr(), nbytes, _stream()))
+    done = parents.new_empty(n, dtype=torch.bool)
+    ws, nbytes = _workspace(0, 0, n, parents)
+    _call(dev, N.load().dpk_page_fork, *st, int(page_size), parents.data_ptr(), children.data_ptr(), n,
+          done.data_ptr(), ws.data_ptr(), nbytes)
     return done
 
 
@@ -359,9 +370,8 @@ def page_trim(page_table: torch.Tensor, kv_lens: torch.Tensor, ref_counts: torch
     n = _vector(rows, "rows")
     if keep is not None:
         _vector(keep, "keep", n)
-    with torch.cuda.device(dev):
-        N.check(N.load().dpk_page_trim(*st, int(page_size), rows.data_ptr(),
-                                       None if keep is None else keep.data_ptr(), n, _stream()))
+    _call(dev, N.load().dpk_page_trim, *st, int(page_size), rows.data_ptr(),
+          None if keep is None else keep.data_ptr(), n)
 
 
 def page_copy(K_pages: torch.Tensor, V_pages: torch.Tensor, src: torch.Tensor, dst: torch.Tensor) -> None:
@@ -372,10 +382,8 @@ def page_copy(K_pages: torch.Tensor, V_pages: torch.Tensor, src: torch.Tensor, d
     pools, P, page = _pools(K_pages, V_pages)
     n = _vector(src, "src")
     _vector(dst, "dst", n)
-    with torch.cuda.device(dev):
-        ws, nbytes = _workspace(0, P, n, dev)
-        N.check(N.load().dpk_page_copy(*pools, P, page, src.data_ptr(), dst.data_ptr(), n,
-                                       ws.data_ptr(), nbytes, _stream()))
+    ws, nbytes = _workspace(0, P, n, src)
+    _call(dev, N.load().dpk_page_copy, *pools, P, page, src.data_ptr(), dst.data_ptr(), n, ws.data_ptr(), nbytes)
 
 
 def page_compact(K_pages: torch.Tensor, V_pages: torch.Tensor, page_table: torch.Tensor,
@@ -388,9 +396,7 @@ def page_compact(K_pages: torch.Tensor, V_pages: torch.Tensor, page_table: torch
     pools, P, page = _pools(K_pages, V_pages)
     if P != st[6]:
         raise ValueError(f"ref_counts has {st[6]} entries, the pools have {P} pages")
-    live = torch.empty(1, dtype=torch.int32, device=dev)
-    with torch.cuda.device(dev):
-        ws, nbytes = _workspace(0, P, 0, dev)
-        N.check(N.load().dpk_page_compact(*pools, *st, page, live.data_ptr(), ws.data_ptr(), nbytes,
-                                          _stream()))
+    live = kv_lens.new_empty(1)
+    ws, nbytes = _workspace(0, P, 0, kv_lens)
+    _call(dev, N.load().dpk_page_compact, *pools, *st, page, live.data_ptr(), ws.data_ptr(), nbytes)
     return live

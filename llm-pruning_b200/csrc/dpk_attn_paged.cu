@@ -725,7 +725,7 @@ extern "C" {
 size_t dpk_attn_paged_workspace_bytes(int64_t N, int S, int Hq, int Hk, int D, int max_query_len, int has_mask)
 {
     if (!paged_sizes_ok(N, S, Hq, Hk, D)) return 0;
-    return paged_shape(N, S, Hq, Hk, D, max_query_len, has_mask != 0, sm_count()).bytes;
+    return paged_shape(N, S, Hq, Hk, D, max_query_len, has_mask != 0, sm_total()).bytes;
 }
 
 int dpk_attn_paged(const void* Q, const void* K, const void* V, const int32_t* page_table,
@@ -754,8 +754,8 @@ int dpk_attn_paged(const void* Q, const void* K, const void* V, const int32_t* p
     DPK_REQUIRE(q_ts % 8 == 0 && kv_ts % 8 == 0 && ps % 8 == 0, "strides must be multiples of 8 elements (16 bytes)");
     DPK_REQUIRE(aligned16(Q) && aligned16(K) && aligned16(V) && aligned16(O), "tensors must be 16-byte aligned");
     if (N == 0) return DPK_OK;
-    const int sms = sm_count();
-    const PagedShape g = paged_shape(N, S, Hq, Hk, D, max_query_len, mask != nullptr, sms);
+    const PagedShape g = paged_shape(N, S, Hq, Hk, D, max_query_len, mask != nullptr, sm_total());
+    const int workers = g.workers / sm_total() * sm_count();      // SMs left free by dpk_set_sm_margin
     const int64_t most = g.max_tiles * ((int64_t(W) * page_size + g.unit_keys - 1) / g.unit_keys + g.tile_gap);
     DPK_REQUIRE(most < (1ll << 31), "too much work for one call: %lld tiles of up to %lld keys",
                 (long long)g.max_tiles, (long long)W * page_size);
@@ -793,14 +793,14 @@ int dpk_attn_paged(const void* Q, const void* K, const void* V, const int32_t* p
     p.part_o = reinterpret_cast<float*>(w + g.off_o);
     p.part_ml = reinterpret_cast<float*>(w + g.off_ml);
     p.tile_rows = g.tile_rows; p.unit_keys = g.unit_keys; p.tile_gap = g.tile_gap;
-    p.workers = g.workers; p.min_range = g.min_range;
+    p.workers = workers; p.min_range = g.min_range;
     p.max_tiles = static_cast<int>(g.max_tiles);
     p.status = device_status_ptr();
     if (!p.status) return fail(DPK_ERR_CUDA, "no status word on this device");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     // workers that can get work at all, as far as the host knows
     int64_t used = (most + g.min_range - 1) / g.min_range;
-    if (used > g.workers) used = g.workers;
+    if (used > workers) used = workers;
     if (used < 1) used = 1;
     const int plan_threads = int64_t(S) * Hk <= 256 && g.max_tiles <= 512 ? 256 : kPlanThreads;
     if (p.rows && S > 0) {

@@ -107,7 +107,7 @@ int make_tmap_2d_plain(CUtensorMap* map, const void* base, uint64_t cols, uint64
 static const int kMaxDev = 64;
 static int g_sm_margin = 0;
 
-int sm_count()
+int sm_total()
 {
     static int cached[kMaxDev] = {0};
     int dev = 0;
@@ -118,7 +118,12 @@ int sm_count()
             n = 148;
         cached[dev] = n;
     }
-    const int usable = cached[dev] - g_sm_margin;
+    return cached[dev];
+}
+
+int sm_count()
+{
+    const int usable = sm_total() - g_sm_margin;
     return usable < 1 ? 1 : usable;
 }
 

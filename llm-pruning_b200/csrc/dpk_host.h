@@ -45,8 +45,11 @@ int make_tmap_3d_sw128(CUtensorMap* map, const void* base, uint64_t cols, uint64
 int make_tmap_2d_plain(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows,
                        uint64_t row_stride_elems, uint32_t box_cols, uint32_t box_rows);
 
-// Number of SMs of the current device (cached per device).
+// Number of SMs of the current device that launches use (cached per device).
 int sm_count();
+
+// The same without the margin of dpk_set_sm_margin: what sizes that outlive a call go by.
+int sm_total();
 
 // Address of the per-device status word kernels report into.
 int* device_status_ptr();

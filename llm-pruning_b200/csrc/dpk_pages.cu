@@ -12,7 +12,9 @@
 // P counts, so these operators run as ONE cluster of eight CTAs: every CTA scans an eighth of the
 // counts, the partial sums meet in distributed shared memory, and no second launch or host round
 // trip is needed between "how many are free" and "who gets which".  They are latency bound (4 bytes
-// per page are read).  The bytes of pages are moved by a second launch over a list the first one
+// per page are read): extending 256 sequences in a pool of 131072 pages takes 14 us.  One CTA instead
+// of eight is as fast up to 262144 pages there (its launch is cheaper, its scan longer) but twice as
+// slow on compacting 65536 and four times on 262144.  The bytes of pages are moved by a second launch over a list the first one
 // wrote, bound by HBM (each byte read once and written once).
 #define DPK_KERNEL_ID 16   // thousands digit of the device status word
 #include <cooperative_groups.h>
@@ -82,11 +84,21 @@ __device__ __forceinline__ int block_scan(int v, int* sh, int& total)
 
 struct ExtendWork {        // workspace, one entry per sequence
     int32_t* tail;         // id of a shared last page that this sequence will write to, else -1
-    int32_t* upto;         // pages needed by the sequences up to and including this one
-    int32_t* need;         // this sequence's own
-    int32_t* keeper;       // 0: nothing shared; 1: copies its tail; 2 + j: keeps it, j = last sharer
+    int32_t* keeper;       // with shared tails: 0 nothing shared; 1 copies its tail; 2 + j: keeps it, j = last sharer
+    int32_t* upto;         // pages needed by the sequences up to and including this one, for more than kPgRows
 };
 
+constexpr int kPgRows = 4096;       // sequences whose running sums fit shared memory
+
+// pages that sequence s will hold with `add` more tokens; more than any table has where that is refused
+__device__ __forceinline__ int64_t pages_wanted(int len, int add, int page)
+{
+    return add < 0 || len < 0 ? INT64_MAX : (static_cast<int64_t>(len) + add + page - 1) / page;
+}
+
+// Every CTA sums up the needs of all sequences for itself (a scan over S, against a round trip through
+// the cluster and one more barrier), so that two cluster barriers are enough: one behind the count
+// of the free pages, one before the lengths change.  Shared tails cost a third.
 __global__ void __cluster_dims__(kPgCluster, 1, 1) __launch_bounds__(kPgThreads)
 page_extend_kernel(const PageState st, const ExtendWork wk, const int32_t* __restrict__ add,
                    uint8_t* __restrict__ granted)
@@ -96,8 +108,10 @@ page_extend_kernel(const PageState st, const ExtendWork wk, const int32_t* __res
     const int gt = rank * kPgThreads + tid;
     constexpr int kAll = kPgCluster * kPgThreads;
     __shared__ int sh[33];
+    __shared__ int sh_upto[kPgRows];
     __shared__ int sh_free;            // free pages of this CTA's slice of the counts
-    __shared__ int sh_used_tails;      // read by rank 0 only: is any tail shared at all
+    __shared__ int sh_shared;          // is any tail of this CTA's rows shared
+    int32_t* upto = st.S <= kPgRows ? sh_upto : wk.upto;    // beyond: every CTA writes the same values
 
     // 1. who writes to a shared, partly filled last page
     if (rank == 0 && tid == 0) *st.count = 0;
@@ -105,9 +119,7 @@ page_extend_kernel(const PageState st, const ExtendWork wk, const int32_t* __res
     for (int s = gt; s < st.S; s += kAll) {
         const int len = st.lens[s], a = add[s];
         int tail = -1;
-        const int64_t want = a < 0 || len < 0 ? INT64_MAX
-                                              : (static_cast<int64_t>(len) + a + st.page - 1) / st.page;
-        if (a > 0 && want <= st.W && len % st.page != 0) {
+        if (a > 0 && len > 0 && len % st.page != 0 && pages_wanted(len, a, st.page) <= st.W) {
             const int id = st.table[s * st.table_stride + pages_of(len, st.page) - 1];
             if (id < 0 || id >= st.P) page_report(st.status);
             else if (st.refs[id] > 1) tail = id;
@@ -115,117 +127,124 @@ page_extend_kernel(const PageState st, const ExtendWork wk, const int32_t* __res
         wk.tail[s] = tail;
         any |= tail >= 0;
     }
-    any = __syncthreads_or(any);
-    if (tid == 0) sh_used_tails = any;
     // free pages of this slice; a slice is a contiguous range of the counts
     const int per = ((st.P + kPgCluster - 1) / kPgCluster + 3) & ~3;
     const int p0 = min(st.P, rank * per), p1 = min(st.P, p0 + per);
     const bool wide = (reinterpret_cast<uintptr_t>(st.refs) & 15u) == 0;
     int mine = 0;
-    for (int p = p0 + tid * 4; p < p1; p += kPgThreads * 4) {
-        if (wide && p + 4 <= p1) {
-            const int4 r = *reinterpret_cast<const int4*>(st.refs + p);
-            mine += (r.x == 0) + (r.y == 0) + (r.z == 0) + (r.w == 0);
-        } else {
-            for (int q = p; q < min(p + 4, p1); ++q) mine += st.refs[q] == 0;
+    if (wide) {
+#pragma unroll 4
+        for (int p = p0 + tid * 4; p < p1; p += kPgThreads * 4) {
+            if (p + 4 <= p1) {
+                const int4 r = *reinterpret_cast<const int4*>(st.refs + p);
+                mine += (r.x == 0) + (r.y == 0) + (r.z == 0) + (r.w == 0);
+            } else {
+                for (int q = p; q < p1; ++q) mine += st.refs[q] == 0;
+            }
         }
+    } else {
+#pragma unroll 8
+        for (int p = p0 + tid; p < p1; p += kPgThreads) mine += st.refs[p] == 0;
     }
+    any = __syncthreads_or(any);
     int total;
     block_scan(mine, sh, total);
-    if (tid == 0) sh_free = total;
+    if (tid == 0) {
+        sh_free = total;
+        sh_shared = any;
+    }
     cluster.sync();
     int shared_tails = 0, before = 0, free_pages = 0;
     for (int r = 0; r < kPgCluster; ++r) {
-        shared_tails |= *cluster.map_shared_rank(&sh_used_tails, r);
+        shared_tails |= *cluster.map_shared_rank(&sh_shared, r);
         const int f = *cluster.map_shared_rank(&sh_free, r);
         free_pages += f;
         if (r < rank) before += f;
     }
 
     // 2. of the sharers of such a page everybody takes a copy, but where all its holders write to
-    //    it the first one keeps it.  Compares every sharer with every row: S^2 / 8192 steps a thread.
-    for (int s = gt; s < st.S; s += kAll) {
-        const int len = st.lens[s], a = add[s];
-        const int64_t want = a < 0 || len < 0 ? INT64_MAX
-                                              : (static_cast<int64_t>(len) + a + st.page - 1) / st.page;
-        int need = want <= st.W ? static_cast<int>(want) - pages_of(len, st.page) : 0;
-        int keep = 0;
-        const int tail = shared_tails ? wk.tail[s] : -1;
-        if (tail >= 0) {
-            int holders = 0, first = s, last = s;
-            for (int j = 0; j < st.S; ++j)
-                if (wk.tail[j] == tail) {
-                    ++holders;
-                    first = min(first, j);
-                    last = max(last, j);
-                }
-            keep = (first == s && holders == st.refs[tail]) ? 2 + last : 1;
+    //    it the first one keeps it.  A warp per sharer compares it with every row.
+    if (shared_tails) {
+        const int lane = tid & 31;
+        for (int s = gt >> 5; s < st.S; s += kAll / 32) {
+            const int tail = wk.tail[s];
+            int keep = 0;
+            if (tail >= 0) {
+                int holders = 0, first = st.S, last = -1;
+#pragma unroll 4
+                for (int j = lane; j < st.S; j += 32)
+                    if (wk.tail[j] == tail) {
+                        ++holders;
+                        first = min(first, j);
+                        last = max(last, j);
+                    }
+                holders = __reduce_add_sync(0xffffffffu, holders);
+                first = __reduce_min_sync(0xffffffffu, first);
+                last = __reduce_max_sync(0xffffffffu, last);
+                keep = (first == s && holders == st.refs[tail]) ? 2 + last : 1;
+            }
+            if (lane == 0) wk.keeper[s] = keep;
         }
-        if (keep == 1) ++need;
-        wk.need[s] = need;
-        wk.keeper[s] = keep;
+        cluster.sync();
     }
-    cluster.sync();
 
-    // 3. running sum of the needs (the first CTA; 1024 rows a step)
-    if (rank == 0) {
-        int carry = 0;
-        for (int s0 = 0; s0 < st.S; s0 += kPgThreads) {
-            const int s = s0 + tid;
-            const int need = s < st.S ? wk.need[s] : 0;
-            int t;
-            const int x = block_scan(need, sh, t);
-            if (s < st.S) wk.upto[s] = carry + x + need;
-            carry += t;
+    // 3. running sum of the needs
+    int wanted = 0;
+    for (int s0 = 0; s0 < st.S; s0 += kPgThreads) {
+        const int s = s0 + tid;
+        int need = 0;
+        if (s < st.S) {
+            const int len = st.lens[s];
+            const int64_t want = pages_wanted(len, add[s], st.page);
+            if (want <= st.W) need = static_cast<int>(want) - pages_of(len, st.page);
+            if (shared_tails) need += wk.keeper[s] == 1;
         }
+        const int x = block_scan(need, sh, total);
+        if (s < st.S) upto[s] = wanted + x + need;
+        wanted += total;
     }
-    cluster.sync();
+    __syncthreads();
 
     // 4. who is granted: in row order while the free pages last
+    auto is_granted = [&](int s, int keep) {
+        if (pages_wanted(st.lens[s], add[s], st.page) > st.W) return false;
+        const int need = upto[s] - (s > 0 ? upto[s - 1] : 0);
+        return (need == 0 || upto[s] <= free_pages) && (keep < 2 || upto[keep - 2] <= free_pages);
+    };
     for (int s = gt; s < st.S; s += kAll) {
-        const int len = st.lens[s], a = add[s], need = wk.need[s], keep = wk.keeper[s];
-        const bool fits = a >= 0 && len >= 0 &&
-                          (static_cast<int64_t>(len) + a + st.page - 1) / st.page <= st.W;
-        bool ok = fits && (need == 0 || wk.upto[s] <= free_pages);
-        if (keep >= 2) ok = ok && wk.upto[keep - 2] <= free_pages;
+        const int keep = shared_tails ? wk.keeper[s] : 0;
+        const bool ok = is_granted(s, keep);
         granted[s] = ok ? 1 : 0;
-        if (!ok) continue;
-        if (keep == 1) {
-            atomicSub(&st.refs[wk.tail[s]], 1);      // its holders stay above zero: see step 2
-        }
+        if (ok && keep == 1) atomicSub(&st.refs[wk.tail[s]], 1);     // its holders stay above zero: see step 2
     }
-    cluster.sync();
 
     // 5. the k-th free page goes to the row whose needs cover k
-    const int wanted = st.S > 0 ? wk.upto[st.S - 1] : 0;
     int base = before;
     for (int c0 = p0; c0 < p1 && base < wanted; c0 += kPgThreads) {
         const int p = c0 + tid;
         const int is_free = p < p1 && st.refs[p] == 0;
-        int t;
-        const int k = base + block_scan(is_free, sh, t);
-        base += t;
+        const int k = base + block_scan(is_free, sh, total);
+        base += total;
         if (!is_free || k >= wanted) continue;
         int lo = 0, hi = st.S - 1;                   // smallest row with upto > k
         while (lo < hi) {
             const int mid = (lo + hi) >> 1;
-            if (wk.upto[mid] > k) hi = mid;
+            if (upto[mid] > k) hi = mid;
             else lo = mid + 1;
         }
-        if (!granted[lo]) continue;
+        const int keep = shared_tails ? wk.keeper[lo] : 0;
+        if (!is_granted(lo, keep)) continue;
         const int len = st.lens[lo], held = pages_of(len, st.page);
-        const int copy = wk.keeper[lo] == 1;
-        const int idx = k - (wk.upto[lo] - wk.need[lo]);
-        const int at = copy ? held - 1 + idx : held + idx;
+        const int idx = k - (lo > 0 ? upto[lo - 1] : 0);
         st.refs[p] = 1;
-        if (copy && idx == 0) {
+        if (keep == 1 && idx == 0) {
             PageMove m;
             m.src = wk.tail[lo];
             m.dst = p;
             m.rows = len % st.page;
             st.moves[atomicAdd(st.count, 1)] = m;
         }
-        st.table[lo * st.table_stride + at] = p;
+        st.table[lo * st.table_stride + held + idx - (keep == 1 ? 1 : 0)] = p;
     }
     cluster.sync();
     for (int s = gt; s < st.S; s += kAll)
@@ -569,7 +588,7 @@ int dpk_page_extend(int32_t* table, int64_t table_stride, int32_t* lens, int32_t
     rc = page_status(st);
     if (rc) return rc;
     int32_t* w = take_moves(st, workspace, S);
-    ExtendWork wk = {w, w + S, w + 2 * S, w + 3 * S};
+    ExtendWork wk = {w, w + S, w + 2 * S};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     page_extend_kernel<<<kPgCluster, kPgThreads, 0, s>>>(st, wk, add, granted);
     DPK_CUDA(cudaGetLastError());

@@ -73,50 +73,50 @@ __device__ __forceinline__ void turn_near(uint4& a, const float2* cs)
     }
 }
 
-constexpr int kRopeThreads = 128;
 constexpr int kRopeMaxPairs = 256;
+constexpr int kRopeWarps = 4;
+constexpr int kRopeFlight = 4;           // heads of a lane in flight
 
-// A CTA per token.  A task is two 16-byte chunks of one head (the two halves of 8 pairs, or 16
-// channels in a row); the loads of a thread's first two tasks are issued before the angles are
-// computed, so the CTA's memory latency hides the sine and cosine.
+// A warp takes one token, or (few tokens) every `split`-th group of its heads.  A lane keeps one place
+// c of a head -- 16 channels: the two halves of 8 pairs, or 16 in a row -- for all the heads it visits,
+// so the 8 angles it needs stay in registers; a warp covers 32 / (D/16) heads per step.  Nothing is
+// shared between warps: one warp's lookups and sines are hidden by the others' copies.  A CTA per
+// token with a barrier between angles and copies measured 130 to 157 us where this takes 114 (16384
+// tokens, 64 + 2 * 8 heads of 128: 5.9 TB/s; 2 heads in flight 117, 8 heads 128).
 template <bool kBf16, bool kNear>
-__global__ void __launch_bounds__(kRopeThreads) rope_paged_kernel(const RopePagedParams p)
+__global__ void __launch_bounds__(kRopeWarps * 32) rope_paged_kernel(const RopePagedParams p, int split)
 {
-    __shared__ float2 cs[kRopeMaxPairs];
-    __shared__ int64_t sh_row;                       // element offset of the token's row in the pools
-    const int tid = threadIdx.x;
-    const int per_head = p.D / 16, rot = p.R / 16;   // tasks of a head, those that turn
+    __shared__ float2 sh_cs[kRopeWarps][kRopeMaxPairs];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float2* cs = sh_cs[warp];
+    const int per_head = p.D / 16, rot = p.R / 16;       // places of a head, those that turn
+    const int across = per_head < 32 ? per_head : 32;    // places of a head that a warp covers at once
+    const int step = 32 / across;                        // heads per step
     const int heads = p.Hq + (p.v ? 2 : 1) * p.Hk;
-    const int tasks = heads * per_head;
-    for (int t = blockIdx.x; t < p.N; t += gridDim.x) {
-        int lo_at, hi_at;
-        auto where = [&](int task, const uint8_t*& src, int& head, int& c) {
-            head = task / per_head;
-            c = task - head * per_head;
-            if (!kNear && c < rot) {
-                lo_at = c * 16;
-                hi_at = p.R + c * 16;                // bytes: R/2 channels further
-            } else {
-                lo_at = c * 32;
-                hi_at = lo_at + 16;
+    const int64_t jobs = static_cast<int64_t>(p.N) * split;
+    const int64_t warps = static_cast<int64_t>(gridDim.x) * kRopeWarps;
+    for (int64_t job = static_cast<int64_t>(blockIdx.x) * kRopeWarps + warp; job < jobs; job += warps) {
+        const int t = static_cast<int>(job / split), part = static_cast<int>(job - static_cast<int64_t>(t) * split);
+        // where the token's k and v go: element offset in the pools, -1 nowhere
+        int64_t row = -1;
+        if (p.k_pages) {
+            if (t >= p.qstart[p.S]) continue;            // behind the last sequence: left as it is
+            int lo = 0, hi = p.S;                        // last sequence that starts at or before t
+            while (hi - lo > 1) {
+                const int width = (hi - lo + 31) / 32, at = lo + lane * width;
+                const bool ok = lane == 0 || (at < hi && p.qstart[at] <= t);
+                const int n = __popc(__ballot_sync(0xffffffffu, ok));
+                hi = min(hi, lo + n * width);
+                lo += (n - 1) * width;
             }
-            if (head < p.Hq) src = p.q + (t * p.q_ts + static_cast<int64_t>(head) * p.D) * 2;
-            else if (head < p.Hq + p.Hk) src = p.k + (t * p.kv_ts + static_cast<int64_t>(head - p.Hq) * p.D) * 2;
-            else src = p.v + (t * p.kv_ts + static_cast<int64_t>(head - p.Hq - p.Hk) * p.D) * 2;
-        };
-        constexpr int kAhead = 2;
-        uint4 a[kAhead], b[kAhead];
-#pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-            const int task = j * kRopeThreads + tid;
-            if (task >= tasks) break;
-            const uint8_t* src;
-            int head, c;
-            where(task, src, head, c);
-            a[j] = *reinterpret_cast<const uint4*>(src + lo_at);
-            b[j] = *reinterpret_cast<const uint4*>(src + hi_at);
+            const int pos = p.kv_lens[lo] - p.qstart[lo + 1] + t;
+            const int w = pos / p.page;
+            const int id = pos >= 0 && w < p.W ? p.table[lo * p.table_stride + w] : -1;
+            if (id >= 0 && id < p.P) row = id * p.page_stride + (pos - w * p.page) * p.token_stride;
+            else if (lane == 0) atomicCAS(p.status, 0, 1000 * DPK_KERNEL_ID + DPK_DEV_BAD_INDEX);   // q is turned all the same
         }
-        for (int i = tid; i < p.R / 2; i += kRopeThreads) {
+        __syncwarp();
+        for (int i = lane; i < p.R / 2; i += 32) {
             int axis = 0;
             if (p.axis_map) {
                 axis = p.axis_map[i];
@@ -135,71 +135,74 @@ __global__ void __launch_bounds__(kRopeThreads) rope_paged_kernel(const RopePage
             sincospif(static_cast<float>(2.0 * (turns - rint(turns))), &s, &c);
             cs[i] = make_float2(c * p.scale, s * p.scale);
         }
-        if (tid == 0) {
-            int64_t row = 0;
-            if (p.k_pages) {
-                row = -1;
-                if (t < p.qstart[p.S]) {
-                    int lo = 0, hi = p.S - 1;        // last sequence that starts at or before t
-                    while (lo < hi) {
-                        const int mid = (lo + hi + 1) >> 1;
-                        if (p.qstart[mid] <= t) lo = mid;
-                        else hi = mid - 1;
+        __syncwarp();
+        for (int cb = 0; cb < per_head; cb += across) {
+            const int c = cb + lane % across;
+            const bool turns = c < rot, busy = lane < step * across && c < per_head;
+            float2 mine[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) mine[k] = turns ? cs[c * 8 + k] : make_float2(1.f, 0.f);
+            const int lo_at = !kNear && turns ? c * 16 : c * 32;
+            const int hi_at = !kNear && turns ? p.R + c * 16 : c * 32 + 16;      // bytes: R/2 channels further
+            const int first = part * step + lane / across, stride = split * step;
+            for (int h0 = first; h0 < heads; h0 += kRopeFlight * stride) {
+                uint4 lo[kRopeFlight], hi[kRopeFlight];
+#pragma unroll
+                for (int k = 0; k < kRopeFlight; ++k) {
+                    const int head = h0 + k * stride;
+                    if (!busy || head >= heads) continue;
+                    const uint8_t* src;
+                    if (head < p.Hq) src = p.q + (t * p.q_ts + static_cast<int64_t>(head) * p.D) * 2;
+                    else if (head < p.Hq + p.Hk) src = p.k + (t * p.kv_ts + static_cast<int64_t>(head - p.Hq) * p.D) * 2;
+                    else src = p.v + (t * p.kv_ts + static_cast<int64_t>(head - p.Hq - p.Hk) * p.D) * 2;
+                    lo[k] = *reinterpret_cast<const uint4*>(src + lo_at);
+                    hi[k] = *reinterpret_cast<const uint4*>(src + hi_at);
+                }
+#pragma unroll
+                for (int k = 0; k < kRopeFlight; ++k) {
+                    const int head = h0 + k * stride;
+                    if (!busy || head >= heads) continue;
+                    if (turns && head < p.Hq + p.Hk) {
+                        if constexpr (kNear) {
+                            turn_near<kBf16>(lo[k], mine);
+                            turn_near<kBf16>(hi[k], mine + 4);
+                        } else {
+                            turn_half<kBf16>(lo[k], hi[k], mine);
+                        }
                     }
-                    const int pos = p.kv_lens[lo] - p.qstart[lo + 1] + t;
-                    const int w = pos / p.page;
-                    const int id = pos >= 0 && w < p.W ? p.table[lo * p.table_stride + w] : -1;
-                    if (id < 0 || id >= p.P) {
-                        atomicCAS(p.status, 0, 1000 * DPK_KERNEL_ID + DPK_DEV_BAD_INDEX);
-                        row = -2;                    // q is turned all the same
+                    uint8_t* dst;
+                    if (head < p.Hq) {
+                        dst = p.q_out + (t * p.qo_ts + static_cast<int64_t>(head) * p.D) * 2;
+                    } else if (!p.k_pages) {
+                        dst = p.k_out + (static_cast<int64_t>(t) * p.Hk + head - p.Hq) * p.D * 2;
+                    } else if (row < 0) {
+                        continue;
+                    } else if (head < p.Hq + p.Hk) {
+                        dst = p.k_pages + (row + static_cast<int64_t>(head - p.Hq) * p.D) * 2;
                     } else {
-                        row = id * p.page_stride + (pos - w * p.page) * p.token_stride;
+                        dst = p.v_pages + (row + static_cast<int64_t>(head - p.Hq - p.Hk) * p.D) * 2;
                     }
+                    *reinterpret_cast<uint4*>(dst + lo_at) = lo[k];
+                    *reinterpret_cast<uint4*>(dst + hi_at) = hi[k];
                 }
             }
-            sh_row = row;
         }
-        __syncthreads();
-        const int64_t row = sh_row;
-        if (row != -1) {                             // -1: behind the last sequence, left as it is
-            for (int j = 0, task = tid; task < tasks; ++j, task += kRopeThreads) {
-                const uint8_t* src;
-                int head, c;
-                where(task, src, head, c);
-                uint4 lo, hi;
-                if (j < kAhead) {
-                    lo = j == 0 ? a[0] : a[1];
-                    hi = j == 0 ? b[0] : b[1];
-                } else {
-                    lo = *reinterpret_cast<const uint4*>(src + lo_at);
-                    hi = *reinterpret_cast<const uint4*>(src + hi_at);
-                }
-                if (head < p.Hq + p.Hk && c < rot) {
-                    if constexpr (kNear) {
-                        turn_near<kBf16>(lo, cs + c * 8);
-                        turn_near<kBf16>(hi, cs + c * 8 + 4);
-                    } else {
-                        turn_half<kBf16>(lo, hi, cs + c * 8);
-                    }
-                }
-                uint8_t* dst;
-                if (head < p.Hq) {
-                    dst = p.q_out + (t * p.qo_ts + static_cast<int64_t>(head) * p.D) * 2;
-                } else if (!p.k_pages) {
-                    dst = p.k_out + (static_cast<int64_t>(t) * p.Hk + head - p.Hq) * p.D * 2;
-                } else if (row < 0) {
-                    continue;
-                } else if (head < p.Hq + p.Hk) {
-                    dst = p.k_pages + (row + static_cast<int64_t>(head - p.Hq) * p.D) * 2;
-                } else {
-                    dst = p.v_pages + (row + static_cast<int64_t>(head - p.Hq - p.Hk) * p.D) * 2;
-                }
-                *reinterpret_cast<uint4*>(dst + lo_at) = lo;
-                *reinterpret_cast<uint4*>(dst + hi_at) = hi;
-            }
-        }
-        __syncthreads();                             // cs and sh_row are written again
     }
+}
+
+template <bool kBf16, bool kNear>
+static void launch_rope(const RopePagedParams& p, cudaStream_t s)
+{
+    // 20 warps fit an SM: fewer tokens than that are split by heads, down to one step a warp; more warps
+    // than fit would only repeat the lookups (2200 tokens: 25 us unsplit, 31 split in two)
+    const int per_head = p.D / 16, step = per_head < 32 ? 32 / per_head : 1;
+    const int heads = p.Hq + (p.v ? 2 : 1) * p.Hk;
+    const int64_t room = static_cast<int64_t>(sm_count()) * 20;
+    int64_t split = room / p.N, most = (heads + step - 1) / step;
+    if (split > most) split = most;
+    if (split < 1) split = 1;
+    const int64_t blocks = (p.N * split + kRopeWarps - 1) / kRopeWarps;
+    rope_paged_kernel<kBf16, kNear><<<static_cast<unsigned>(blocks), kRopeWarps * 32, 0, s>>>(p, static_cast<int>(split));
 }
 
 }  // namespace dpk
@@ -280,15 +283,13 @@ extern "C" int dpk_rope_append_paged(const void* q, const void* k, const void* v
     p.wide_positions = positions_64 ? 1 : 0;
     p.status = device_status_ptr();
     if (!p.status) return fail(DPK_ERR_CUDA, "no status word on this device");
-    const int cap = sm_count() * 16;
-    const unsigned blocks = static_cast<unsigned>(N < cap ? N : cap);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == DPK_BF16) {
-        if (neighbours) rope_paged_kernel<true, true><<<blocks, kRopeThreads, 0, s>>>(p);
-        else rope_paged_kernel<true, false><<<blocks, kRopeThreads, 0, s>>>(p);
+        if (neighbours) launch_rope<true, true>(p, s);
+        else launch_rope<true, false>(p, s);
     } else {
-        if (neighbours) rope_paged_kernel<false, true><<<blocks, kRopeThreads, 0, s>>>(p);
-        else rope_paged_kernel<false, false><<<blocks, kRopeThreads, 0, s>>>(p);
+        if (neighbours) launch_rope<false, true>(p, s);
+        else launch_rope<false, false>(p, s);
     }
     DPK_CUDA(cudaGetLastError());
     return DPK_OK;

@@ -15,6 +15,7 @@ their range are reported through :func:`dpk_b200.ops.device_status` and never fo
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -158,7 +159,7 @@ def attention_paged(Q: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tenso
     Qc, q_ts = _token_rows(Q)
     clear = 0
     if O is None:
-        O = Q.new_empty((n, Hq, D))
+        O = torch.empty_like(Q, memory_format=torch.contiguous_format)
         clear = 1
     elif O.shape != Q.shape or O.dtype != Q.dtype or not O.is_contiguous():
         raise ValueError("O must be contiguous with the shape and dtype of Q")
@@ -166,7 +167,12 @@ def attention_paged(Q: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tenso
     if n and most < 1:
         raise ValueError("max_query_len must be at least 1")
     lib = N.load()
-    nbytes = lib.dpk_attn_paged_workspace_bytes(n, S, Hq, Hk, D, most, 0 if m8 is None else 1)
+    with_mask = 0 if m8 is None else 1
+    if torch.cuda.current_device() == dev:
+        nbytes = _attention_workspace_bytes(dev, n, S, Hq, Hk, D, most, with_mask)
+    else:
+        with torch.cuda.device(dev):
+            nbytes = _attention_workspace_bytes(dev, n, S, Hq, Hk, D, most, with_mask)
     ws = page_table.new_empty((nbytes + 3) // 4)
     _call(dev, lib.dpk_attn_paged,
           Qc.data_ptr(), K_pages.data_ptr(), V_pages.data_ptr(), page_table.data_ptr(), kv_lens.data_ptr(),
@@ -174,6 +180,12 @@ def attention_paged(Q: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tenso
           Hk, D, NG, D ** -0.5 if scale is None else float(scale), 1 if is_causal else 0, code,
           most if most > 1 else 1, clear, q_ts, ps, ts, tstride, ws.data_ptr(), nbytes)
     return O, {}
+
+
+@functools.lru_cache(maxsize=64)
+def _host_ints(values: tuple):
+    """A host array of C ints (never written to)."""
+    return (ctypes.c_int32 * len(values))(*values)
 
 
 def _rope(dev, q, k, v, positions, inv_freq, sections, axis_map, interleaved, attention_scale, q_out, cache):
@@ -207,7 +219,7 @@ def _rope(dev, q, k, v, positions, inv_freq, sections, axis_map, interleaved, at
     elif sections is not None:
         if len(sections) != axes:
             raise ValueError(f"{len(sections)} sections for {axes} axes")
-        secs = (ctypes.c_int32 * axes)(*[int(x) for x in sections])
+        secs = _host_ints(tuple(map(int, sections)))
     elif axes > 1:
         raise ValueError("several axes need sections or axis_map")
     qc, q_ts = _token_rows(q)
@@ -219,7 +231,7 @@ def _rope(dev, q, k, v, positions, inv_freq, sections, axis_map, interleaved, at
             kc, vc = k.contiguous(), v.contiguous()
             kv_ts = Hk * D
     if q_out is None:
-        q_out = q.new_empty((n, Hq, D))
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         qo_ts = Hq * D
     else:
         if q_out.shape != q.shape or q_out.dtype != q.dtype:
@@ -229,7 +241,7 @@ def _rope(dev, q, k, v, positions, inv_freq, sections, axis_map, interleaved, at
             raise ValueError("q_out: the heads of a token must be contiguous, 16-byte aligned")
     k_out = None
     if cache is None:
-        k_out = q.new_empty((n, Hk, D))
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
         tail = (None, None, 0, 0, None, 0, None, None, n, 0, 0, 0, 0)
     else:
         k_pages, v_pages, page_table, kv_lens, query_start = cache
@@ -305,16 +317,29 @@ def _pools(k_pages, v_pages):
     if k_pages.dim() != 5 or k_pages.element_size() != 2:
         raise ValueError("pools must be 16-bit [layers, pages, page_size, kv_heads, head_dim]")
     L, P, page, Hk, D = k_pages.shape
-    if P and not k_pages[0, 0].is_contiguous():
-        raise ValueError("a page must be contiguous")
+    ls, ps, ts, hs, es = k_pages.stride()
     row = Hk * D
-    ps = k_pages.stride(1) if P > 1 else page * row
-    ls = k_pages.stride(0) if L > 1 else 0
+    if (es != 1 and D > 1) or (hs != D and Hk > 1) or (ts != row and page > 1):
+        raise ValueError("a page must be contiguous")
+    if P <= 1:
+        ps = page * row
+    if L <= 1:
+        ls = 0
     return (k_pages.data_ptr(), v_pages.data_ptr(), L, ls, ps, row), P, page
 
 
+@functools.lru_cache(maxsize=256)
+def _page_workspace_bytes(S: int, P: int, n: int) -> int:
+    return N.load().dpk_page_workspace_bytes(S, P, n)
+
+
+@functools.lru_cache(maxsize=256)
+def _attention_workspace_bytes(dev: int, *sizes: int) -> int:
+    return N.load().dpk_attn_paged_workspace_bytes(*sizes)
+
+
 def _workspace(S: int, P: int, n: int, like: torch.Tensor):
-    nbytes = N.load().dpk_page_workspace_bytes(S, P, n)
+    nbytes = _page_workspace_bytes(S, P, n)
     return like.new_empty((nbytes + 3) // 4), nbytes
 
 

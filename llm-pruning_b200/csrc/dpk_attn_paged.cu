@@ -40,17 +40,18 @@ __device__ __forceinline__ int2 plan_scan(int2 v, int2* sh, int2& total)
     __syncthreads();                       // the previous use of sh is over
     if (lane == 31) sh[warp] = x;
     __syncthreads();
-    int2 w = lane < warps ? sh[lane] : make_int2(0, 0);
-    int2 before = make_int2(0, 0);
-    total = make_int2(0, 0);
+    if (warp == 0) {
+        int2 w = lane < warps ? sh[lane] : make_int2(0, 0);
 #pragma unroll
-    for (int k = 0; k < 32; ++k) {
-        if (k >= warps) break;
-        const int y = __shfl_sync(0xffffffffu, w.x, k), z = __shfl_sync(0xffffffffu, w.y, k);
-        if (k < warp) { before.x += y; before.y += z; }
-        total.x += y;
-        total.y += z;
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, w.x, o), z = __shfl_up_sync(0xffffffffu, w.y, o);
+            if (lane >= o) { w.x += y; w.y += z; }
+        }
+        sh[lane] = w;
     }
+    __syncthreads();
+    total = sh[warps - 1];
+    const int2 before = warp ? sh[warp - 1] : make_int2(0, 0);
     return make_int2(x.x - v.x + before.x, x.y - v.y + before.y);
 }
 
@@ -77,18 +78,27 @@ __global__ void __launch_bounds__(1024) paged_rows_kernel(const PagedParams p)
     int tok0;
     const int total_rows = plan_new(p, s, tok0) * p.rep;
     int32_t* out = p.rows + (static_cast<int64_t>(kvh) * p.N + tok0) * p.rep;
+    const int g0 = kvh * p.rep / p.hpg, h0 = kvh * p.rep - g0 * p.hpg;
     int carry = 0;
     for (int x0 = 0; x0 < total_rows; x0 += blockDim.x * 16) {
         const int x = x0 + threadIdx.x * 16;
         uint32_t on = 0;
         if (x < total_rows) {
-            int i = x / p.rep, r = x - i * p.rep;
+            const int i = x / p.rep;
+            int r = x - i * p.rep;
+            int g = (kvh * p.rep + r) / p.hpg, h = kvh * p.rep + r - g * p.hpg;   // group and place in it
             const uint8_t* m = p.mask + static_cast<int64_t>(tok0 + i) * p.NG;
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
-                if (x + k < total_rows && m[(kvh * p.rep + r) / p.hpg] != 0) on |= 1u << k;
+                if (x + k < total_rows && m[g] != 0) on |= 1u << k;
+                if (++h == p.hpg) {
+                    h = 0;
+                    ++g;
+                }
                 if (++r == p.rep) {
                     r = 0;
+                    g = g0;
+                    h = h0;
                     m += p.NG;
                 }
             }

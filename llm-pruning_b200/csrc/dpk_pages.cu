@@ -103,6 +103,7 @@ __global__ void __cluster_dims__(kPgCluster, 1, 1) __launch_bounds__(kPgThreads)
 page_extend_kernel(const PageState st, const ExtendWork wk, const int32_t* __restrict__ add,
                    uint8_t* __restrict__ granted)
 {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = static_cast<int>(cluster.block_rank()), tid = threadIdx.x;
     const int gt = rank * kPgThreads + tid;
@@ -341,6 +342,7 @@ __global__ void __cluster_dims__(kPgCluster, 1, 1) __launch_bounds__(kPgThreads)
 page_copy_list_kernel(const PageState st, const int32_t* __restrict__ src, const int32_t* __restrict__ dst,
                       int n, int32_t* __restrict__ mark)
 {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     cg::cluster_group cluster = cg::this_cluster();
     const int gt = static_cast<int>(cluster.block_rank()) * kPgThreads + threadIdx.x;
     constexpr int kAll = kPgCluster * kPgThreads;
@@ -378,6 +380,7 @@ __global__ void __cluster_dims__(kPgCluster, 1, 1) __launch_bounds__(kPgThreads)
 page_compact_kernel(const PageState st, int32_t* __restrict__ remap, int32_t* __restrict__ holes,
                     int32_t* __restrict__ live_out)
 {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = static_cast<int>(cluster.block_rank()), tid = threadIdx.x;
     __shared__ int sh[33];
@@ -439,6 +442,8 @@ page_compact_kernel(const PageState st, int32_t* __restrict__ remap, int32_t* __
 __global__ void __launch_bounds__(256)
 page_remap_kernel(const PageState st, const int32_t* __restrict__ remap, const int32_t* __restrict__ live)
 {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int limit = *live;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
          i < static_cast<int64_t>(st.S) * st.W; i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
@@ -467,6 +472,7 @@ __global__ void __launch_bounds__(256)
 page_move_kernel(const PageMove* __restrict__ moves, const int32_t* __restrict__ count, const PoolParams pp,
                  int page)
 {
+    asm volatile("griddepcontrol.wait;" ::: "memory");       // started while the bookkeeping still runs
     const int pieces = (page * pp.row_bytes + kMoveBytes - 1) / kMoveBytes;
     const int64_t tasks = static_cast<int64_t>(*count) * pp.layers * 2 * pieces;
     for (int64_t i = blockIdx.x; i < tasks; i += gridDim.x) {
@@ -495,11 +501,26 @@ page_move_kernel(const PageMove* __restrict__ moves, const int32_t* __restrict__
     }
 }
 
+// A launch that may start while the one before it on the stream still runs; its kernel waits for that one.
+template <class... KArgs, class... Args>
+static int launch_early(int64_t blocks, void (*kernel)(KArgs...), cudaStream_t s, Args... args)
+{
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+    cfg.blockDim = dim3(256);
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    DPK_CUDA(cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...));
+    return DPK_OK;
+}
+
 static int move_pages(const PageState& st, const PoolParams& pp, cudaStream_t s)
 {
-    page_move_kernel<<<sm_count() * 8, 256, 0, s>>>(st.moves, st.count, pp, st.page);
-    DPK_CUDA(cudaGetLastError());
-    return DPK_OK;
+    return launch_early(sm_count() * 8, page_move_kernel, s, st.moves, st.count, pp, st.page);
 }
 
 static int pool_params(PoolParams& pp, void* k, void* v, int layers, int64_t layer_stride, int64_t page_stride,
@@ -683,8 +704,8 @@ int dpk_page_compact(void* k, void* v, int layers, int64_t layer_stride, int64_t
     if (S > 0 && W > 0) {
         int64_t blocks = (static_cast<int64_t>(S) * W + 255) / 256;
         if (blocks > sm_count() * 8) blocks = sm_count() * 8;
-        page_remap_kernel<<<static_cast<unsigned>(blocks), 256, 0, s>>>(st, remap, live);
-        DPK_CUDA(cudaGetLastError());
+        rc = launch_early(blocks, page_remap_kernel, s, st, remap, live);
+        if (rc) return rc;
     }
     return move_pages(st, pp, s);
 }

@@ -68,7 +68,41 @@ __device__ __forceinline__ int plan_new(const PagedParams& p, int s, int& tok0)
     return end - tok0;
 }
 
-// Active rows of every (sequence, KV head), in token order; used where tiles have many rows, so that
+// Tile number `at` of an item of `rows` rows, and the units of its visible range.
+__device__ __forceinline__ int plan_tile(const PagedParams& p, int seq, int kvh, int at, int rows, PagedTile& t)
+{
+    t.seq = seq;
+    t.kvh = kvh;
+    const int fresh = plan_new(p, seq, t.tok0);
+    t.m0 = at * p.tile_rows;
+    t.rows = min(p.tile_rows, rows - t.m0);
+    t.kv_len = p.kv_lens[seq];
+    if (t.kv_len < 0 || t.kv_len > static_cast<int64_t>(p.W) * p.page) {
+        atomicCAS(p.status, 0, 1000 * DPK_KERNEL_ID + DPK_DEV_BAD_INDEX);
+        t.kv_len = 0;
+    }
+    t.pos0 = t.kv_len - fresh;
+    t.kv_end = t.kv_len;
+    int last = 0, head;
+    if (p.rows || !p.mask) {
+        if (p.causal) last = paged_row(p, t, t.rows - 1, head);
+    } else {                                     // the last row that is not routed out
+        last = -1;
+        for (int r = t.rows - 1; r >= 0 && last < 0; --r) last = paged_row(p, t, r, head);
+    }
+    if (p.causal) t.kv_end = min(t.kv_len, t.pos0 + last + 1);
+    return last >= 0 && t.kv_end > 0 ? paged_units(p, t) : 0;
+}
+
+// Where the tiles of (s, kvh) are put down by paged_rows_kernel: room for as many as its rows can need.
+__device__ __forceinline__ int plan_slot(const PagedParams& p, int s, int kvh)
+{
+    int tok0;
+    const int fresh = plan_new(p, s, tok0);
+    return p.Hk * (tok0 * p.rep / p.tile_rows + s) + kvh * (fresh * p.rep / p.tile_rows + 1);
+}
+
+// Active rows of every (sequence, KV head), in token order, and its tiles; used where tiles have many rows, so that
 // none of them is spent on a routed-out (token, head).  A thread looks at 16 rows in a row.
 __global__ void __launch_bounds__(1024) paged_rows_kernel(const PagedParams p)
 {
@@ -109,6 +143,13 @@ __global__ void __launch_bounds__(1024) paged_rows_kernel(const PagedParams p)
         carry += t.x;
     }
     if (threadIdx.x == 0) p.row_count[s * p.Hk + kvh] = carry;
+    __syncthreads();
+    PagedTile* slot = p.slot + plan_slot(p, s, kvh);
+    for (int t = threadIdx.x; t * p.tile_rows < carry; t += blockDim.x) {
+        PagedTile pt;
+        if (plan_tile(p, s, kvh, t, carry, pt) == 0) pt.kv_end = 0;
+        slot[t] = pt;
+    }
 }
 
 // The whole block cuts the work: `tile`, `start` [tiles + 1] and `first` [S * Hk] may be shared memory.
@@ -148,8 +189,8 @@ __device__ __forceinline__ void plan_work(const PagedParams& p, PagedTile* tile,
         int n = 0;
         PagedTile pt = {};
         if (q < tiles) {
-            const int g = static_cast<int>((static_cast<int64_t>(q + 1) * p.workers - 1) / tiles);
-            const int g_first = static_cast<int>(static_cast<int64_t>(g) * tiles / p.workers), k = q - g_first;
+            // max_tiles * workers < 2^31 was checked
+            const int g = ((q + 1) * p.workers - 1) / tiles, g_first = g * tiles / p.workers, k = q - g_first;
             const int t = k < rounds ? k * p.workers + g : rounds * p.workers + g_first - g * rounds;
             int lo = 0, hi = items - 1;
             while (lo < hi) {                        // last item that starts at or before t
@@ -157,28 +198,14 @@ __device__ __forceinline__ void plan_work(const PagedParams& p, PagedTile* tile,
                 if (first[mid] <= t) lo = mid;
                 else hi = mid - 1;
             }
-            pt.seq = lo / p.Hk;
-            pt.kvh = lo - pt.seq * p.Hk;
-            const int fresh = plan_new(p, pt.seq, pt.tok0);
-            const int rows = p.rows ? p.row_count[lo] : fresh * p.rep;
-            pt.m0 = (t - first[lo]) * p.tile_rows;
-            pt.rows = min(p.tile_rows, rows - pt.m0);
-            pt.kv_len = p.kv_lens[pt.seq];
-            if (pt.kv_len < 0 || pt.kv_len > static_cast<int64_t>(p.W) * p.page) {
-                atomicCAS(p.status, 0, 1000 * DPK_KERNEL_ID + DPK_DEV_BAD_INDEX);
-                pt.kv_len = 0;
+            const int s = lo / p.Hk, kvh = lo - s * p.Hk;
+            if (p.rows) {
+                pt = p.slot[plan_slot(p, s, kvh) + t - first[lo]];
+                n = paged_units(p, pt);
+            } else {
+                int tok0;
+                n = plan_tile(p, s, kvh, t - first[lo], plan_new(p, s, tok0) * p.rep, pt);
             }
-            pt.pos0 = pt.kv_len - fresh;
-            pt.kv_end = pt.kv_len;
-            int last = 0, head;
-            if (p.rows || !p.mask) {
-                if (p.causal) last = paged_row(p, pt, pt.rows - 1, head);
-            } else {                                 // the last row that is not routed out
-                last = -1;
-                for (int r = pt.rows - 1; r >= 0 && last < 0; --r) last = paged_row(p, pt, r, head);
-            }
-            if (p.causal) pt.kv_end = min(pt.kv_len, pt.pos0 + last + 1);
-            if (last >= 0 && pt.kv_end > 0) n = paged_units(p, pt);
         }
         int2 total;
         const int2 at = plan_scan(make_int2(n > 0, n > 0 ? n + p.tile_gap : 0), sh, total);
@@ -499,12 +526,12 @@ __global__ void __launch_bounds__(kPwWarps * 32) paged_warp_kernel(const PagedPa
 
 // ---- joining -----------------------------------------------------------------------------------
 
-// The first join_blocks = workers * row_groups blocks join the tiles that several workers shared: block
+// The last join_blocks = workers * row_groups blocks join the tiles that several workers shared: block
 // (w, g) takes a share of the rows of the tile that starts in worker w's range and ends behind it.
 // Where that are up to eight parts a warp joins kRows rows by itself, their loads in flight
-// together; else the block's four warps share the parts of each row.  The other blocks write the
+// together; else the block's four warps share the parts of each row.  The blocks before write the
 // rows that no unit covers, a token per warp: routed out, without a visible key, and (clear_tail)
-// behind the last sequence.
+// behind the last sequence.  They need nothing of the attention kernel, so they do not wait for it.
 struct JoinRow {
     float m, l;
 };
@@ -537,9 +564,11 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p, in
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     __shared__ float sh_o[4][D];
     __shared__ float2 sh_ml[4];
-    paged_wait_previous();
-    if (static_cast<int>(blockIdx.x) < join_blocks) {
-        const int w0 = blockIdx.x / row_groups, group = blockIdx.x - w0 * row_groups;
+    const int zero_blocks = gridDim.x - join_blocks;
+    if (static_cast<int>(blockIdx.x) >= zero_blocks) {
+        paged_wait_previous();
+        const int block = blockIdx.x - zero_blocks;
+        const int w0 = block / row_groups, group = block - w0 * row_groups;
         const PagedBorder border = p.border[w0];
         const PagedTile& t = border.tile;
         const int w1 = border.last_worker, slot0 = border.slot;
@@ -621,7 +650,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p, in
         }
         return;
     }
-    for (int t = (blockIdx.x - join_blocks) * 4 + warp; t < p.N; t += (gridDim.x - join_blocks) * 4) {
+    for (int t = blockIdx.x * 4 + warp; t < p.N; t += zero_blocks * 4) {
         const bool tail = p.S == 0 || t >= p.qstart[p.S];
         if (tail && !p.clear_tail) continue;
         int seen = -1;                                       // last key the token sees
@@ -640,11 +669,21 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p, in
                    : p.causal ? min(len - 1, len - p.qstart[lo + 1] + t) : len - 1;
         }
         if (seen >= 0 && !p.mask) continue;
-        for (int x = lane; x < p.Hq * (D / 8); x += 32) {
-            const int head = x / (D / 8);
-            if (seen < 0 || p.mask[static_cast<int64_t>(t) * p.NG + head / p.hpg] == 0)
-                *reinterpret_cast<uint4*>(p.O + (static_cast<int64_t>(t) * p.Hq * D + x * 8) * 2) =
-                    make_uint4(0, 0, 0, 0);
+        constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;     // lanes of a head's row, rows of a store
+        uint8_t* out = p.O + static_cast<int64_t>(t) * p.Hq * D * 2;
+        for (int h0 = 0; h0 < p.Hq; h0 += 32) {
+            const int h = h0 + lane;
+            uint32_t dead = __ballot_sync(0xffffffffu, h < p.Hq && (seen < 0 ||
+                                          p.mask[static_cast<int64_t>(t) * p.NG + h / p.hpg] == 0));
+            while (dead) {
+                uint32_t mine = dead;
+                for (int k = 0; k < lane / kLanes; ++k) mine &= mine - 1;
+                if (mine)
+                    *reinterpret_cast<uint4*>(out + ((h0 + __ffs(mine) - 1) * D + lane % kLanes * 8) * 2) =
+                        make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int k = 0; k < kAtOnce; ++k) dead &= dead - 1;
+            }
         }
     }
 }
@@ -696,7 +735,7 @@ struct PagedShape {
     int tile_rows, unit_keys, tile_gap, workers, min_range;
     int64_t max_tiles;
     bool plan_here;
-    size_t off_start, off_tile, off_first, off_rows, off_count, off_border, off_o, off_ml, bytes;
+    size_t off_start, off_tile, off_slot, off_first, off_rows, off_count, off_border, off_o, off_ml, bytes;
 };
 
 static PagedShape paged_shape(int64_t N, int S, int Hq, int Hk, int D, int max_query_len, bool has_mask, int sms)
@@ -720,6 +759,7 @@ static PagedShape paged_shape(int64_t N, int S, int Hq, int Hk, int D, int max_q
         return here;
     };
     g.off_tile = take(size_t(g.max_tiles) * sizeof(PagedTile));
+    g.off_slot = take(g.tc && has_mask ? size_t(g.max_tiles) * sizeof(PagedTile) : 0);
     g.off_start = take(size_t(g.max_tiles + 1) * 4);
     g.off_first = take(size_t(S) * Hk * 4);
     g.off_rows = take(g.tc && has_mask ? size_t(Hk) * N * rep * 4 : 0);
@@ -779,6 +819,7 @@ int dpk_attn_paged(const void* Q, const void* K, const void* V, const int32_t* p
     const int64_t most = g.max_tiles * ((int64_t(W) * page_size + g.unit_keys - 1) / g.unit_keys + g.tile_gap);
     DPK_REQUIRE(most < (1ll << 31), "too much work for one call: %lld tiles of up to %lld keys",
                 (long long)g.max_tiles, (long long)W * page_size);
+    DPK_REQUIRE((g.max_tiles + 1) * g.workers < (1ll << 31), "too many tiles for one call");
     DPK_REQUIRE(int64_t(Hq) * N < (1ll << 31), "too many rows for one call");
     DPK_REQUIRE(workspace && workspace_bytes >= g.bytes, "workspace of %zu bytes needed, %zu given", g.bytes,
                 workspace_bytes);
@@ -805,6 +846,7 @@ int dpk_attn_paged(const void* Q, const void* K, const void* V, const int32_t* p
     uint8_t* w = static_cast<uint8_t*>(workspace);
     p.head = reinterpret_cast<PagedHead*>(w);
     p.tile = reinterpret_cast<PagedTile*>(w + g.off_tile);
+    p.slot = reinterpret_cast<PagedTile*>(w + g.off_slot);
     p.start = reinterpret_cast<int32_t*>(w + g.off_start);
     p.first_tile = reinterpret_cast<int32_t*>(w + g.off_first);
     p.rows = g.tc && mask ? reinterpret_cast<int32_t*>(w + g.off_rows) : nullptr;

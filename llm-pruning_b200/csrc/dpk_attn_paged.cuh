@@ -59,6 +59,7 @@ struct PagedParams {
     PagedHead* head;
     int32_t* start;         // [tiles + 1] place of each tile's first unit
     PagedTile* tile;        // [tiles]
+    PagedTile* slot;        // [max_tiles] with `rows`: tiles as paged_rows_kernel leaves them
     int32_t* first_tile;    // [S * Hk + 1] running number of tiles before dropping empty ones
     int32_t* rows;          // [Hk][N * rep] active rows of each (sequence, KV head), or NULL: all rows
     int32_t* row_count;     // [S * Hk] with `rows`
@@ -69,13 +70,21 @@ struct PagedParams {
     int* status;
 };
 
-// Row r of a tile's list -> new token and query head; -1 where the row is routed out.
+// Row r of a tile's list -> new token and query head; -1 where the row is routed out.  The bounds hold
+// by themselves as long as query_start ascends; where it does not, two sequences may have written
+// over each other's lists, and the checks keep every access inside Q, O and the lists.
 __device__ __forceinline__ int paged_row(const PagedParams& p, const PagedTile& t, int r, int& head)
 {
     int x = t.m0 + r;
-    if (p.rows) x = p.rows[(static_cast<int64_t>(t.kvh) * p.N + t.tok0) * p.rep + x];
+    head = t.kvh * p.rep;
+    if (p.rows) {
+        const int64_t at = static_cast<int64_t>(t.tok0) * p.rep + x;
+        if (at >= static_cast<int64_t>(p.N) * p.rep) return -1;
+        x = p.rows[static_cast<int64_t>(t.kvh) * p.N * p.rep + at];
+    }
     const int i = x / p.rep;
-    head = t.kvh * p.rep + (x - i * p.rep);
+    if (t.tok0 + i >= p.N) return -1;
+    head += x - i * p.rep;
     if (!p.rows && p.mask && p.mask[static_cast<int64_t>(t.tok0 + i) * p.NG + head / p.hpg] == 0) return -1;
     return i;
 }

@@ -382,6 +382,23 @@ def test_attention_paged_is_registered():
     assert dpk_b200.get_kernel("attention_paged", arch="sm100").backend == "b200"
 
 
+@pytest.mark.gpu
+def test_attention_paged_starts_that_do_not_ascend_are_reported(ops):
+    """Overlapping and backward sequences: nothing outside the tensors is touched, and the status says so."""
+    b = make([200, 150, 100], [20, 30, 40], 16, 8, 2, 64, BF, seed=21)
+    d = cuda(b)
+    mask = (torch.rand(450, 2, generator=b["gen"]) < 0.7).cuda()
+    guard = torch.full((452, 8, 64), 5.0, dtype=BF, device="cuda")
+    for start in ([0, 300, 100, 450], [0, 450, 0, 450], [450, 0, 450, 450], [-3, 200, 350, 450], [0, 200, 451, 450]):
+        st = torch.tensor(start, dtype=torch.int32, device="cuda")
+        for m in (mask, None):
+            for most in (1, 200):
+                ops.attention_paged(d["q"], d["k"], d["v"], d["table"], d["lens"], st, m, O=guard[1:451],
+                                    max_query_len=most)
+                assert ops.device_status() % 1000 == 105
+    assert (guard[0] == 5).all() and (guard[451] == 5).all()
+
+
 # ------------------------------------------------------------------------------------ rope (GPU)
 
 ROPE = [

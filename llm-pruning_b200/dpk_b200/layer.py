@@ -114,6 +114,16 @@ class RoutedDecoderLayer:
         if B != 1:
             meta = {}        # per-batch layout (attention) vs flattened layout (GEMMs)
         self._mark("attn")
+        out, fm, fm_all = self._after_attention(x, attn, am, meta)
+        if return_masks == "full":
+            return out, am_all, fm_all
+        return (out, am, fm) if return_masks else out
+
+    def _after_attention(self, x: torch.Tensor, attn: torch.Tensor, am: torch.Tensor, meta: dict):
+        """Output projection, skip connections, second router + norm and FFN: ``(layer output, this rank's
+        FFN mask, the mask of all groups)``."""
+        f = self.front
+        B, T, _ = x.shape
         if self.sum_o is not None:
             x1 = self.sum_o.routed_gemm_k(attn.view(B, T, self.Hq * self.D), self.wo, am,
                                           residual=x.contiguous())
@@ -140,9 +150,37 @@ class RoutedDecoderLayer:
             else:
                 out = self.ffn(h2, fm, events=self.ffn_events, residual=x1)
         self._mark("ffn")
+        return out, fm, fm_all
+
+    def forward_cached(self, x: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, cache,
+                       layer: int, query_start: torch.Tensor, max_query_len: Optional[int] = None,
+                       return_masks: bool = False, **rope):
+        """:meth:`forward_full` for the new tokens of many sequences over a paged cache
+        (:class:`dpk_b200.wide.PagedKVCache`, its ``extend`` called for this step): prompt chunks, single
+        tokens and drafts side by side.  ``x [N,H]``, the new tokens back to back (``query_start``);
+        ``positions [axes,N]`` or ``[N]`` and ``inv_freq`` as :func:`ops.rope_append_paged` takes them, with
+        its ``sections`` / ``axis_map`` / ``interleaved`` / ``attention_scale``; ``layer``: this layer's
+        number in the cache."""
+        f = self.front
+        N = x.shape[0]
+        x3 = x[None]
+        self._mark("start")
+        am, h, _ = ops.router_norm(x3, *f["attn"], norm_weight=f["n1"], eps=f["eps"])
+        am_all = am
+        if f["ar"] is not None:
+            am = am[..., f["ar"][0]:f["ar"][1]]
+        self._mark("route1")
+        q, k, v = self.project_qkv(h, am)
+        # rows of routed-out head groups were not projected: they are turned as they are and never attended
+        q = cache.rope_update(layer, q[0], k[0], v[0], positions, inv_freq, query_start, q_out=q[0], **rope)
+        self._mark("qkv")
+        attn = cache.attend(layer, q, query_start, am[0], max_query_len=max_query_len,
+                            out=self._attention_out(1, N, q)[0])
+        self._mark("attn")
+        out, fm, fm_all = self._after_attention(x3, attn[None], am, {})
         if return_masks == "full":
-            return out, am_all, fm_all
-        return (out, am, fm) if return_masks else out
+            return out[0], am_all[0], fm_all[0]
+        return (out[0], am[0], fm[0]) if return_masks else out[0]
 
     def project_qkv(self, h: torch.Tensor, attn_mask: torch.Tensor):
         """``q [B,T,Hq,D]``, ``k, v [B,T,Hk,D]`` of ``h [B,T,H]``; rows of q whose head group is

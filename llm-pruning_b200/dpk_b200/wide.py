@@ -189,3 +189,76 @@ class SeqFirstKVCache:
                                           self.keys, self.values, self.length)
         self.length += key_states.shape[1]
         return q, keys, values
+
+
+class PagedKVCache:
+    """Keys and values of many sequences of different lengths in pages of one pool, for all layers.
+
+    Paged counterpart of :class:`SeqFirstKVCache`: sequences grow one by one (``extend``), share what they
+    have in common (``fork``: nothing is copied until one of them writes), shrink (``trim``: drafted
+    tokens that were refused) and end (``free``) without moving one another.  All state lives on the
+    GPU and is never read back, so a whole serving step can be captured into a graph:
+
+    * ``page_table [max_sequences, ceil(max_length / page_size)]`` int32, ``lengths [max_sequences]`` int32,
+      ``ref_counts [pages]`` int32;
+    * ``keys, values [layers, pages, page_size, num_kv_heads, head_dim]``.
+
+    A step: ``granted = cache.extend(add)``; per layer ``q = cache.rope_update(layer, q, k, v, ...)`` and
+    ``o = cache.attend(layer, q, ...)`` with the new tokens of all sequences back to back, those of
+    row ``s`` at ``query_start[s] .. query_start[s+1]-1`` (as many as ``add[s]``; a row that was not granted
+    must bring none).  No reference counterpart (its cache is one contiguous tensor per layer,
+    ``WIDE/wrapper/cache.py:10-60``)."""
+
+    def __init__(self, layers: int, pages: int, page_size: int, num_kv_heads: int, head_dim: int,
+                 max_sequences: int, max_length: int, dtype: torch.dtype, device):
+        if page_size <= 0 or page_size % 8:
+            raise ValueError(f"page_size {page_size} must be a multiple of 8")
+        shape = (layers, pages, page_size, num_kv_heads, head_dim)
+        self.keys = torch.empty(shape, dtype=dtype, device=device)
+        self.values = torch.empty(shape, dtype=dtype, device=device)
+        ints = dict(dtype=torch.int32, device=device)
+        self.page_table = torch.full((max_sequences, -(-max_length // page_size)), -1, **ints)
+        self.lengths = torch.zeros(max_sequences, **ints)
+        self.ref_counts = torch.zeros(pages, **ints)
+        self.page_size = page_size
+
+    def extend(self, add: torch.Tensor) -> torch.Tensor:
+        """Room for ``add [max_sequences]`` more tokens; ``granted`` bool (:func:`ops.page_extend`)."""
+        return ops.page_extend(self.keys, self.values, self.page_table, self.lengths, self.ref_counts, add)
+
+    def fork(self, parents: torch.Tensor, children: torch.Tensor) -> torch.Tensor:
+        """Empty rows ``children`` share everything of rows ``parents`` (:func:`ops.page_fork`)."""
+        return ops.page_fork(self.page_table, self.lengths, self.ref_counts, parents, children, self.page_size)
+
+    def trim(self, rows: torch.Tensor, keep: torch.Tensor) -> None:
+        """Sequences ``rows`` keep their first ``keep`` tokens (:func:`ops.page_trim`)."""
+        ops.page_trim(self.page_table, self.lengths, self.ref_counts, rows, keep, page_size=self.page_size)
+
+    def free(self, rows: torch.Tensor) -> None:
+        """Sequences ``rows`` end."""
+        ops.page_trim(self.page_table, self.lengths, self.ref_counts, rows, page_size=self.page_size)
+
+    def compact(self) -> torch.Tensor:
+        """Moves the held pages to the front of the pool; their number, int32 ``[1]`` (:func:`ops.page_compact`)."""
+        return ops.page_compact(self.keys, self.values, self.page_table, self.lengths, self.ref_counts)
+
+    def rope_update(self, layer: int, query_states: torch.Tensor, key_states: torch.Tensor,
+                    value_states: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
+                    query_start: torch.Tensor, **kw) -> torch.Tensor:
+        """Writes the rotated keys and the values of the new tokens into ``layer`` and returns the rotated
+        queries (:func:`ops.rope_append_paged`; ``sections``, ``axis_map``, ``interleaved``,
+        ``attention_scale``, ``q_out`` pass through)."""
+        return ops.rope_append_paged(query_states, key_states, value_states, positions, inv_freq, self.keys[layer],
+                                     self.values[layer], self.page_table, self.lengths, query_start, **kw)
+
+    def attend(self, layer: int, query_states: torch.Tensor, query_start: torch.Tensor,
+               execute_attn: Optional[torch.Tensor] = None, scaling: Optional[float] = None,
+               is_causal: bool = True, max_query_len: Optional[int] = None,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """:func:`routed_attention` of the new tokens ``[N,Hq,D]`` over everything cached of their sequence;
+        ``execute_attn [N,groups]`` (or ``[N]``) 0/1 of any dtype, ``None`` = every head."""
+        if execute_attn is not None and execute_attn.dim() == 1:
+            execute_attn = execute_attn[:, None]
+        return ops.attention_paged(query_states, self.keys[layer], self.values[layer], self.page_table,
+                                   self.lengths, query_start, execute_attn, O=out, scale=scaling,
+                                   is_causal=is_causal, max_query_len=max_query_len)[0]

@@ -686,3 +686,177 @@ def test_page_extend_many_pages_and_rows(ops):
     add = torch.randint(0, 30, (S,), generator=g).tolist()
     c.extend(ops, add)
     assert c.table.tolist() == c.books.table and c.refs.tolist() == c.books.refs and c.lens.tolist() == c.books.lens
+
+
+# ----------------------------------------------------------------- the operators together (GPU)
+
+@pytest.mark.gpu
+def test_serving_run_over_a_paged_cache(ops):
+    """Prompts in chunks, single tokens, forks, drafts that are refused, sequences that end, a compacted
+    pool -- with the attention of every step checked against keys and values kept per sequence."""
+    from dpk_b200.wide import PagedKVCache
+
+    g = torch.Generator().manual_seed(31)
+    rng = random.Random(31)
+    S, L, Hq, Hk, D, NG, page = 6, 2, 8, 2, 64, 4, 8
+    cache = PagedKVCache(L, 90, page, Hk, D, S, 200, BF, "cuda")
+    inv = (10000.0 ** (-torch.arange(D // 2, dtype=torch.float64) / (D // 2))).float().cuda()
+    kept = [[([], []) for _ in range(L)] for _ in range(S)]       # per row and layer: keys, values
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    lens = lambda: [len(kept[s][0][0]) for s in range(S)]
+
+    def step(add):
+        granted = cache.extend(i32(add)).tolist()
+        add = [a if ok else 0 for a, ok in zip(add, granted)]
+        starts = [0]
+        for a in add:
+            starts.append(starts[-1] + a)
+        n = starts[-1]
+        if n == 0:
+            return granted
+        base = lens()
+        pos = torch.tensor([[base[s] + i for s in range(S) for i in range(add[s])],
+                            [rng.randrange(40) for _ in range(n)]]).cuda()
+        for layer in range(L):
+            q, k, v = (torch.randn(n, h, D, generator=g).to(BF).cuda() for h in (Hq, Hk, Hk))
+            mask = torch.rand(n, NG, generator=g) < 0.7
+            kr = ops.rope_axes(q, k, pos, inv, (20, 12))[1].cpu()
+            qr = cache.rope_update(layer, q, k, v, pos, inv, i32(starts), sections=(20, 12))
+            out = cache.attend(layer, qr, i32(starts), mask.to(BF).cuda(), max_query_len=max(add))
+            for s in range(S):
+                for i in range(add[s]):
+                    kept[s][layer][0].append(kr[starts[s] + i])
+                    kept[s][layer][1].append(v[starts[s] + i].cpu())
+                if add[s] == 0:
+                    continue
+                ks, vs = (torch.stack(t)[None] for t in kept[s][layer])          # one page per sequence
+                a, b = starts[s], starts[s + 1]
+                one = dict(q=qr[a:b].cpu(), k=ks, v=vs, table=torch.zeros(1, 1, dtype=torch.int32),
+                           lens=torch.tensor([ks.shape[1]]), start=torch.tensor([0, b - a]))
+                check_attention(out[a:b], one, mask[a:b])
+        assert cache.lengths.tolist() == lens()
+        return granted
+
+    def fork(parents, children):
+        assert cache.fork(i32(parents), i32(children)).all()
+        for p, c in zip(parents, children):
+            kept[c] = [(list(k), list(v)) for k, v in kept[p]]
+
+    def trim(rows, keep):
+        cache.trim(i32(rows), i32(keep))
+        for s, n in zip(rows, keep):
+            for k, v in kept[s]:
+                del k[n:], v[n:]
+
+    assert all(step([20, 33, 0, 0, 8, 0]))
+    assert all(step([17, 1, 0, 0, 1, 0]))                # a chunk beside single tokens
+    fork([0, 1, 0], [2, 3, 5])
+    assert all(step([1] * 6))                            # everybody writes: tails are copied
+    assert all(step([4] * 6))                            # drafts ...
+    trim([0, 2, 3], [lens()[0] - 4, lens()[2] - 3, 11])  # ... refused, one far into what it shares
+    assert all(step([1] * 6))
+    cache.free(i32([1]))
+    kept[1] = [([], []) for _ in range(L)]
+    live = cache.compact()
+    assert int(live) == int((cache.ref_counts > 0).sum()) and (cache.ref_counts[int(live):] == 0).all()
+    assert all(step([2, 50, 1, 1, 1, 1]))
+    assert not all(step([100, 100, 100, 150, 150, 150]))  # more than the pool has
+    step([1] * 6)
+    cache.free(i32(list(range(S))))
+    assert (cache.ref_counts == 0).all() and (cache.page_table == -1).all()
+
+
+@pytest.mark.gpu
+def test_decoder_layer_over_a_paged_cache(ops):
+    """RoutedDecoderLayer.forward_cached: two sequences in chunks of many and of single tokens, against the
+    oracle composition of each whole sequence with the masks that the layer decided."""
+    from dpk_b200.layer import RoutedDecoderLayer
+    from dpk_b200.wide import PagedKVCache
+    from oracle import dpk_oracle as O
+
+    g = torch.Generator().manual_seed(43)
+    H, Hq, Hk, D, I, NGF, R = 256, 8, 2, 64, 1024, 8, 16
+    r16 = lambda t: t.to(BF).float()
+    rand = lambda *shape, std=1.0: r16(torch.randn(*shape, generator=g) * std)
+    ws = {n: rand(*shp, std=0.05) for n, shp in dict(wq=(Hq * D, H), wk=(Hk * D, H), wv=(Hk * D, H),
+                                                     wo=(H, Hq * D), wg=(I, H), wu=(I, H), wd=(H, I)).items()}
+    router = lambda ng: (rand(R, H, std=H ** -0.5), rand(R, std=0.1), rand(2 * ng, R, std=R ** -0.5), rand(2 * ng, std=0.1))
+    ra, rf = router(Hk), router(NGF)
+    n1, n2 = r16(1 + 0.1 * torch.randn(H, generator=g)), r16(1 + 0.1 * torch.randn(H, generator=g))
+    gpu = lambda t: t.to(BF).cuda()
+    layer = RoutedDecoderLayer(*(gpu(ws[n]) for n in ("wq", "wk", "wv", "wo", "wg", "wu", "wd")), num_q_heads=Hq,
+                               num_kv_heads=Hk, head_dim=D, attn_groups=Hk, ffn_groups=NGF, max_tokens=400)
+    layer.set_front_end(tuple(map(gpu, ra)), tuple(map(gpu, rf)), gpu(n1), gpu(n2), 1e-5)
+    cache = PagedKVCache(3, 60, 16, Hk, D, 2, 320, BF, "cuda")
+    inv = (10000.0 ** (-torch.arange(D // 2, dtype=torch.float64) / (D // 2))).float()
+    xs = [rand(190, H), rand(131, H)]
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    outs, masks = [[], []], [[], []]
+    at = [0, 0]
+    for add in ([150, 0], [30, 129], [1, 1], [9, 1]):
+        assert cache.extend(i32(add)).all()
+        x = torch.cat([xs[s][at[s]:at[s] + add[s]] for s in range(2)])
+        pos = torch.tensor([at[s] + i for s in range(2) for i in range(add[s])])
+        out, am, fm = layer.forward_cached(gpu(x), pos.cuda(), inv.cuda(), cache, 1, i32([0, add[0], sum(add)]),
+                                           max_query_len=max(add), return_masks=True)
+        for s in range(2):
+            a = sum(add[:s])
+            outs[s].append(out[a:a + add[s]].float().cpu())
+            masks[s].append((am[a:a + add[s]].cpu(), fm[a:a + add[s]].cpu()))
+            at[s] += add[s]
+    for s in range(2):
+        T = xs[s].shape[0]
+        x, am, fm = xs[s][None], torch.cat([m[0] for m in masks[s]])[None], torch.cat([m[1] for m in masks[s]])[None]
+        axis = [0] * (D // 2)
+        pos = torch.arange(T)
+        turn = lambda t: r16(PO.rotate(t, pos, inv, axis)[0].float())
+        h = O.rms_norm(x.to(BF), n1, 1e-5).float()
+        q = turn(r16(O.gemm_mn(h, ws["wq"], am)).view(T, Hq, D))[None]
+        k = turn(r16(h @ ws["wk"].T).view(T, Hk, D))[None]
+        v = r16(h @ ws["wv"].T).view(1, T, Hk, D)
+        a = r16(O.attention_prefill(q, k, v, am)).view(1, T, Hq * D)
+        x1 = r16(x + r16(O.gemm_k(a, ws["wo"], am)))
+        h2 = O.rms_norm(x1.to(BF), n2, 1e-5).float()
+        want = x1 + O.ffn_swiglu(h2, ws["wg"], ws["wu"], ws["wd"], fm, round_intermediate=BF)
+        # the tolerance of the same chain without a cache (test_routed_decoder_layer_full_front_end)
+        assert O.rel_err(torch.cat(outs[s])[None], want) <= 3e-2
+    assert ops.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_decode_step_in_one_graph(ops):
+    """extend, rotary write and attention captured together: every replay is one more token."""
+    from dpk_b200.wide import PagedKVCache
+
+    g = torch.Generator().manual_seed(51)
+    S, Hq, Hk, D, page = 3, 4, 2, 64, 8
+    cache = PagedKVCache(1, 30, page, Hk, D, S, 64, BF, "cuda")
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    add, start = i32([1] * S), i32(list(range(S + 1)))
+    q, k, v = (torch.zeros(S, h, D, dtype=BF, device="cuda") for h in (Hq, Hk, Hk))
+    inv = torch.ones(D // 2, device="cuda")
+
+    def step():
+        cache.extend(add)
+        qr = cache.rope_update(0, q, k, v, (cache.lengths - 1)[None], inv, start)
+        return qr, cache.attend(0, qr, start, max_query_len=1)
+    step()
+    cache.free(i32(list(range(S))))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        qr, out = step()
+    keys, values = [[] for _ in range(S)], [[] for _ in range(S)]
+    for n in range(1, 21):
+        for t in (q, k, v):
+            t.copy_(torch.randn(t.shape, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert cache.lengths.tolist() == [n] * S
+        kr = ops.rope_axes(q, k, torch.full((1, S), n - 1, device="cuda"), inv)[1].cpu()
+        for s in range(S):
+            keys[s].append(kr[s])
+            values[s].append(v[s].cpu())
+            one = dict(q=qr[s:s + 1].cpu(), k=torch.stack(keys[s])[None], v=torch.stack(values[s])[None],
+                       table=torch.zeros(1, 1, dtype=torch.int32), lens=torch.tensor([n]), start=torch.tensor([0, 1]))
+            check_attention(out[s:s + 1], one)

@@ -10,6 +10,8 @@ and its fraction of the measured roofline.
     python -m dpk_b200.perf --kernel attention_prefill      # 8192-token routed prefill attention
     python -m dpk_b200.perf --kernel attention_decode       # decode step, batch 64, 32768-token KV cache
     python -m dpk_b200.perf --kernel ffn_decode             # decode-step FFN, 64 tokens
+    python -m dpk_b200.perf --kernel attention_paged        # 4096 new tokens over 12288 in pages of 64
+    python -m dpk_b200.perf --kernel attention_paged --batch 64   # decode step over pages of 16
     python -m dpk_b200.perf --kernel gemm_mn | gemm_k | ffn # Llama-3-8B-shaped FFN prefill and its two GEMMs
 """
 
@@ -287,11 +289,44 @@ def run_gemm_k_scatter(args):
                          "note": "executed flops (the masked formulation runs 2x the algorithmic ones)"}}
 
 
+def run_paged(args):
+    """Attention over a paged cache: one sequence's chunk of new tokens, or with ``--batch`` a decode
+    step (one new token per sequence over 16384 cached ones)."""
+    S = args.batch or 1
+    new, page = (1, 16) if args.batch else (args.tokens or 4096, 64)
+    cached = (args.tokens or 16384) - 1 if args.batch else 12288
+    Hq, Hk, D, NG, keep = 32, 8, 128, 8, 4
+    gen = torch.Generator(device="cuda").manual_seed(SEED)
+    bf = torch.float16 if args.fp16 else torch.bfloat16
+    per = -(-(new + cached) // page)
+    k = torch.randn(S * per, page, Hk, D, generator=gen, device="cuda", dtype=bf)
+    v = torch.randn(S * per, page, Hk, D, generator=gen, device="cuda", dtype=bf)
+    table = torch.randperm(S * per, generator=gen, device="cuda").to(torch.int32).view(S, per)
+    q = torch.randn(S * new, Hq, D, generator=gen, device="cuda").to(bf)
+    lens = torch.full((S,), new + cached, dtype=torch.int32, device="cuda")
+    start = torch.arange(S + 1, dtype=torch.int32, device="cuda") * new
+    mask = topk_mask((S * new, NG), keep, gen)
+    out = torch.empty_like(q)
+    ms, lo, hi = time_ms(lambda: ops.attention_paged(q, k, v, table, lens, start, mask, O=out,
+                                                     max_query_len=new), args.reps)
+    peak_tf, peak_gbs, src = peaks()
+    if args.batch:
+        work = 2.0 * D * 2 * (new + cached) * int(mask.sum())      # NG == Hk: one group per KV head
+        ach, roof = work / (ms * 1e-3) / 1e9, dict(bound="hbm", peak=peak_gbs, unit="GB/s", peak_source=src + " copy bandwidth")
+    else:
+        seen = torch.arange(cached + 1, cached + new + 1, device="cuda", dtype=torch.float64)
+        work = 4.0 * D * float((mask.to(torch.float64) * seen[:, None]).sum()) * (Hq // NG)
+        ach, roof = work / (ms * 1e-3) / 1e12, dict(bound="tensor", peak=peak_tf, unit="TFLOP/s", peak_source=src + " sustained bf16")
+    return {"kernel": "attention_paged", "workload": f"{S} sequence(s), {new} new token(s) over {cached} cached in pages "
+            f"of {page}, Hq={Hq} Hk={Hk} D={D}, top-{keep} of {NG} head groups", "ms": ms, "ms_q20": lo, "ms_q80": hi,
+            "roofline": dict(roof, achieved=ach, frac=ach / roof["peak"])}
+
+
 def main(argv=None):
     ap = argparse.ArgumentParser(description=__doc__)
     ap.add_argument("--kernel", required=True,
                     choices=["attention_prefill", "attention_decode", "ffn", "ffn_decode",
-                             "gemm_mn", "gemm_k", "router_norm", "gemm_k_scatter"])
+                             "gemm_mn", "gemm_k", "router_norm", "gemm_k_scatter", "attention_paged"])
     ap.add_argument("--hidden", type=int, default=0, help="override the hidden size (router_norm)")
     ap.add_argument("--reps", type=int, default=20)
     ap.add_argument("--tokens", type=int, default=0, help="override the token / KV length")
@@ -326,6 +361,8 @@ def main(argv=None):
         res = run_router_norm(args)
     elif args.kernel == "gemm_k_scatter":
         res = run_gemm_k_scatter(args)
+    elif args.kernel == "attention_paged":
+        res = run_paged(args)
     else:
         res = run_gemm(args, args.kernel)
     status = ops.device_status()

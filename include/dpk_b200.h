@@ -384,7 +384,7 @@ int dpk_rope_append(void* q, void* k, const void* v, const void* cos, const void
  * that a token may not see but another new token of its sequence may: finite values only).
  * max_query_len: an upper bound of n_s.  It chooses the kernel and the size of the workspace; a
  * sequence with more new tokens than it says is still computed.
- * Requirements: D in {64,128}, Hq % Hk == 0, Hq/Hk <= 128, Hq % NG == 0, page_size % 8 == 0.
+ * Requirements: D in {64,128}, Hq % Hk == 0, Hq/Hk <= 128, Hq % NG == 0, page_size % 8 == 0, scale > 0.
  */
 size_t dpk_attn_paged_workspace_bytes(int64_t N, int S, int Hq, int Hk, int D, int max_query_len,
                                       int has_mask);

@@ -19,6 +19,8 @@
 #define DPK_KERNEL_ID 13   // thousands digit of the device status word
 #include "dpk_attn_paged.cuh"
 
+#include <math.h>
+
 namespace dpk {
 
 // ---- the work list -------------------------------------------------------------------------------
@@ -805,6 +807,8 @@ int dpk_attn_paged(const void* Q, const void* K, const void* V, const int32_t* p
     DPK_REQUIRE(page_size > 0 && page_size % 8 == 0, "page_size %d must be a multiple of 8", page_size);
     DPK_REQUIRE(int64_t(W) * page_size < (1ll << 30), "a row of the table holds 2^30 tokens or more");
     DPK_REQUIRE(max_query_len >= 1, "max_query_len must be at least 1");
+    // the running maximum is one of q.k, so the scale may not turn its order round; 0 * -inf is no score
+    DPK_REQUIRE(scale > 0.f && scale < INFINITY, "scale must be positive and finite");
     const int64_t q_ts = q_token_stride ? q_token_stride : int64_t(Hq) * D;
     const int64_t kv_ts = page_token_stride ? page_token_stride : int64_t(Hk) * D;
     const int64_t ps = page_stride ? page_stride : page_size * kv_ts;

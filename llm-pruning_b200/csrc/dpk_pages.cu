@@ -557,7 +557,8 @@ static int page_state(PageState& st, int32_t* table, int64_t table_stride, int32
     DPK_REQUIRE(S >= 0 && W >= 0 && P >= 0 && page > 0, "bad shape");
     DPK_REQUIRE(table_stride >= W, "table_stride is smaller than a row");
     DPK_REQUIRE(static_cast<int64_t>(W) * page < (1ll << 31), "a row of the table holds 2^31 tokens or more");
-    DPK_REQUIRE(P <= (1 << 30) && S <= (1 << 24), "too many pages or sequences");
+    DPK_REQUIRE(P <= (1 << 30) && S <= (1 << 24) && static_cast<int64_t>(S) * (W + 1) < (1ll << 31),
+                "too many pages or sequences");
     st.table = table;
     st.table_stride = table_stride;
     st.lens = lens;

@@ -166,6 +166,10 @@ def attention_paged(Q: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tenso
     most = n if max_query_len is None else int(max_query_len)
     if n and most < 1:
         raise ValueError("max_query_len must be at least 1")
+    if n == 0 or S == 0:                 # nothing to attend: every row is behind the last sequence
+        if clear:
+            O.zero_()
+        return O, {}
     lib = N.load()
     with_mask = 0 if m8 is None else 1
     if torch.cuda.current_device() == dev:
@@ -253,8 +257,12 @@ def _rope(dev, q, k, v, positions, inv_freq, sections, axis_map, interleaved, at
         S, W, tstride = _table(page_table)
         _ints(kv_lens, (S,), "kv_lens")
         _ints(query_start, (S + 1,), "query_start")
+        if S == 0:
+            return q_out, None
         tail = (k_pages.data_ptr(), v_pages.data_ptr(), ps, ts, page_table.data_ptr(), tstride,
                 kv_lens.data_ptr(), query_start.data_ptr(), n, S, W, P, page)
+    if n == 0:
+        return q_out, k_out
     _call(dev, N.load().dpk_rope_append_paged,
           qc.data_ptr(), kc.data_ptr(), None if vc is None else vc.data_ptr(), q_out.data_ptr(),
           None if k_out is None else k_out.data_ptr(), q_ts, kv_ts, qo_ts, positions.data_ptr(), axis_stride,
@@ -281,7 +289,8 @@ def rope_append_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positio
     len(inv_freq)`` of the head's channels turn and the others pass through.  A pair is channels
     ``(i, R/2+i)``, with ``interleaved`` channels ``(2i, 2i+1)``; ``attention_scale`` multiplies cos
     and sin.  A token's place in the cache is its place in the sequence (the last tokens of
-    ``kv_lens[s]``), whatever its rotary positions.  Counterpart of :func:`rope_append`; computed
+    ``kv_lens[s]``), whatever its rotary positions.  Rows behind ``query_start[S]`` are not touched (in a
+    new ``q`` they hold anything).  Counterpart of :func:`rope_append`; computed
     from positions, so far ones keep their exact angle."""
     dev = _on_gpu(q, k, v, positions, inv_freq, K_pages, V_pages, page_table, kv_lens, query_start, axis_map, q_out)
     return _rope(dev, q, k, v, positions, inv_freq, sections, axis_map, interleaved, attention_scale, q_out,

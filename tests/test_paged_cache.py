@@ -106,13 +106,14 @@ def test_c_entries_refuse_before_any_launch(ops):
     buf = (ctypes.c_uint8 * 4096)()
     p = (ctypes.addressof(buf) + 255) & ~255
 
-    def attn(N_=4, S=2, W=4, P=8, page=16, Hq=8, Hk=2, D=128, NG=2, most=1, mask=p, ws=0, q_ts=0, ts=0, ps=0):
-        return lib.dpk_attn_paged(p, p, p, p, p, p, mask, p, N_, S, W, P, page, Hq, Hk, D, NG, 0.1, 1, N.BF16,
+    def attn(N_=4, S=2, W=4, P=8, page=16, Hq=8, Hk=2, D=128, NG=2, most=1, mask=p, ws=0, q_ts=0, ts=0, ps=0, sc=0.1):
+        return lib.dpk_attn_paged(p, p, p, p, p, p, mask, p, N_, S, W, P, page, Hq, Hk, D, NG, sc, 1, N.BF16,
                                   most, 0, q_ts, ps, ts, 0, p, ws, None)
     for kw, word in ((dict(D=96), "head_dim"), (dict(Hq=7), "multiple of Hk"), (dict(NG=3), "multiple of NG"),
                      (dict(page=12), "page_size"), (dict(page=0), "page_size"), (dict(most=0), "max_query_len"),
                      (dict(Hq=258, Hk=2, mask=None), "128"), (dict(q_ts=8), "strides"), (dict(ts=257), "strides"),
-                     (dict(W=1 << 28, page=8), "2\\^30"), (dict(), "workspace")):
+                     (dict(W=1 << 28, page=8), "2\\^30"), (dict(sc=0.0), "scale"), (dict(sc=-1.0), "scale"),
+                     (dict(sc=math.inf), "scale"), (dict(sc=math.nan), "scale"), (dict(), "workspace")):
         rc = attn(**kw)
         assert rc == N.ERR_INVALID, kw
         with pytest.raises(ValueError, match=word):
@@ -136,6 +137,8 @@ def test_c_entries_refuse_before_any_launch(ops):
     assert rc == N.ERR_INVALID and "workspace" in N.last_error()
     rc = lib.dpk_page_extend(p, 3, p, p, 2, 4, 8, 16, p, p, p, p, 1, 0, 2048, 128, p, 4096, None)
     assert rc == N.ERR_INVALID and "table_stride" in N.last_error()
+    rc = lib.dpk_page_extend(p, 4096, p, p, 1 << 20, 4096, 8, 16, p, p, p, p, 1, 0, 2048, 128, p, 1 << 40, None)
+    assert rc == N.ERR_INVALID and "too many" in N.last_error()
     rc = lib.dpk_page_fork(p, 4, p, p, 2, 4, 8, 0, p, p, 1, p, p, 4096, None)
     assert rc == N.ERR_INVALID
     rc = lib.dpk_page_copy(p, p, 1, 0, 104, 128, 8, 16, p, p, 1, p, 4096, None)
@@ -377,6 +380,72 @@ def test_attention_paged_in_a_graph_follows_the_state(ops, most):
         check_attention(out, c)
 
 
+@pytest.mark.gpu
+def test_attention_paged_of_nothing_and_through_the_registry(ops):
+    import dpk_b200
+    b = make([1, 40], [30, 9], 16, 4, 2, 64, BF, seed=22)
+    d = cuda(b)
+    got, meta = dpk_b200.run_kernel("attention_paged", d["q"], d["k"], d["v"], d["table"], d["lens"], d["start"])
+    check_attention(got, b)
+    none = torch.zeros(3, dtype=torch.int32, device="cuda")
+    out, _ = ops.attention_paged(d["q"][:0], d["k"], d["v"], d["table"], d["lens"], none)
+    assert out.shape == (0, 4, 64)
+    out, _ = ops.attention_paged(d["q"], d["k"], d["v"], d["table"], d["lens"], none)
+    assert (out == 0).all()                                # every token is behind the last sequence
+    out, _ = ops.attention_paged(d["q"], d["k"], d["v"], d["table"][:0], d["lens"][:0], none[:1])
+    assert (out == 0).all()
+    inv, pos = torch.ones(32, device="cuda"), torch.zeros(1, 0, dtype=torch.int64, device="cuda")
+    assert ops.rope_append_paged(d["q"][:0], d["q"][:0, :2], d["q"][:0, :2], pos, inv, d["k"], d["v"], d["table"],
+                                 d["lens"], none).shape == (0, 4, 64)
+    assert torch.equal(d["k"].cpu(), b["k"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("most", [1, 64])
+def test_attention_paged_beside_other_work(ops, most):
+    """Two calls at once on two streams, and calls that leave SMs to others."""
+    from dpk_b200 import _native as N
+    bs = [make([30, 2, 1] * 4, [700, 3, 90] * 4, 16, 8, 2, 128, BF, seed=23 + i) for i in range(2)]
+    ds = [cuda(b) for b in bs]
+    streams = [torch.cuda.Stream() for _ in bs]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                d = ds[i]
+                outs[i].append(ops.attention_paged(d["q"], d["k"], d["v"], d["table"], d["lens"], d["start"],
+                                                   max_query_len=most)[0])
+    torch.cuda.synchronize()
+    for i, b in enumerate(bs):
+        check_attention(outs[i][0], b)
+        assert all(torch.equal(o, outs[i][0]) for o in outs[i])
+    N.check(N.load().dpk_set_sm_margin(100))
+    try:
+        d = ds[0]
+        got, _ = ops.attention_paged(d["q"], d["k"], d["v"], d["table"], d["lens"], d["start"], max_query_len=most)
+        check_attention(got, bs[0])
+    finally:
+        N.check(N.load().dpk_set_sm_margin(0))
+
+
+@pytest.mark.gpu
+def test_attention_paged_many_tiles_per_worker_and_many_parts_per_tile(ops):
+    """600 sequences of a few tokens (several tiles per worker), then one sequence and one KV head over a
+    long cache (every worker has a part of the one tile)."""
+    new = [1 + i % 3 for i in range(600)]
+    b = make(new, [i * 7 % 90 for i in range(600)], 8, 4, 2, 64, FP, seed=25)
+    d = cuda(b)
+    for most in (1, 3, 40):
+        got, _ = ops.attention_paged(d["q"], d["k"], d["v"], d["table"], d["lens"], d["start"], max_query_len=most)
+        check_attention(got, b)
+    b = make([3], [40000], 32, 8, 1, 64, BF, seed=26)
+    d = cuda(b)
+    for most in (1, 3):
+        got, _ = ops.attention_paged(d["q"], d["k"], d["v"], d["table"], d["lens"], d["start"], max_query_len=most)
+        check_attention(got, b)
+
+
 def test_attention_paged_is_registered():
     import dpk_b200
     assert dpk_b200.get_kernel("attention_paged", arch="sm100").backend == "b200"
@@ -410,6 +479,8 @@ ROPE = [
     ([33], [100], 8, 64, 8, 128, 128, 2, False, FP),
     ([5, 6], [1, 2], 16, 2, 1, 96, 48, 3, False, BF),
     ([9], [0], 16, 1, 1, 32, 16, 1, False, FP),
+    ([3, 2], [5, 0], 8, 2, 1, 768, 512, 2, False, BF),      # a head wider than a warp covers at once
+    ([3, 2], [5, 0], 8, 3, 1, 1024, 272, 1, True, FP),
 ]
 
 

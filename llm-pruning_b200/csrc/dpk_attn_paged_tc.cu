@@ -9,13 +9,18 @@
 //     O += P V       UMMA 128 x D x 64, A = P from TMEM, V in its natural [key][d] layout
 // O is rescaled only when a row's maximum has grown by more than 2^8.
 //
-// K and V arrive by TMA through a map [page][row of page][Hk * D] whose box is gcd(page_size, 64) rows
-// by 64 channels: a unit is put together from as many boxes as pages meet in it, each lane of the
-// producer warp looking up and loading its own (one lane that issues all of them is slower: 721 us
-// instead of 540 for 4096 tokens over 12288 in pages of 16).  Boxes behind the tile's last visible key get a page
-// number outside the map and arrive as zeros; rows of V behind it inside a box (whatever a page holds
-// behind its sequence) are cleared in shared memory by the softmax warps before the product, since
-// 0 * NaN would not be 0.  Their K needs nothing: those scores are replaced by -inf.
+// K and V arrive by TMA through a map [page][64-channel block][row of page][64] whose box is gcd(page_size,
+// 64) rows of one or both blocks: a unit is put together from as many boxes as pages meet in it, each
+// lane of the producer warp looking up and loading its own (one lane that issues all of them is slower:
+// 721 us instead of 526 for 4096 tokens over 12288 in pages of 16, with a box per block).  The copy engine needs some 30 cycles
+// a box whatever its size, so a box takes both blocks of a head where the operand can be read that way:
+// always for V, whose product steps through the rows 16 at a time, and for K where the 8-row groups of a
+// block stay equally spaced (boxes of 8 or of 64 rows): 494 us instead of 526 for those 4096 tokens in
+// pages of 16, 530 instead of 717 in pages of 8, 457 in pages of 64.
+// Boxes behind the tile's last visible key get a page number outside the map and arrive as zeros; rows
+// of V behind it inside a box (whatever a page holds behind its sequence) are cleared in shared memory by
+// the softmax warps before the product, since 0 * NaN would not be 0.  Their K needs nothing: those
+// scores are replaced by -inf.
 //
 // Warp roles (192 threads): 0-3 softmax and epilogue, 4 producer, 5 UMMA issuer and TMEM owner.
 // 96 KiB of shared memory and 256 TMEM columns: two CTAs share an SM and fill each other's gaps.
@@ -36,13 +41,16 @@ struct PtSmem {
     static constexpr int kTotal = kOffBar + 16 * 8 + 16;
 };
 
-template <int D, bool kBf16>
+// kBox: rows of a box where that is known at compile time (64: one box a unit), else 0.
+template <int D, bool kBf16, int kBox>
 __global__ void __launch_bounds__(kPtThreads, 2)
 paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                const PagedParams p, const int box_rows)
+                const PagedParams p, const int box, const bool whole)
 {
     using L = PtSmem<D>;
     constexpr int KBQ = D / 64;
+    const int box_rows = kBox ? kBox : box;
+    const bool k_whole = kBox == 64 || whole;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* sQ = smem + L::kOffQ;
     uint8_t* sK = smem + L::kOffK;
@@ -172,8 +180,9 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                     uint8_t* v = sV + sb * L::kKV;
                     for (int x = threadIdx.x; x < (r1 - r0) * KBQ * 8; x += 128) {
                         const int r = r0 + x / (KBQ * 8), c = x % (KBQ * 8);
-                        *reinterpret_cast<uint4*>(v + (c >> 3) * (kPtBN * 128) + r * 128 + (c & 7) * 16) =
-                            make_uint4(0, 0, 0, 0);
+                        const int which = r / box_rows, in_box = r - which * box_rows;
+                        *reinterpret_cast<uint4*>(v + (which * KBQ + (c >> 3)) * (box_rows * 128) + in_box * 128 +
+                                                  (c & 7) * 16) = make_uint4(0, 0, 0, 0);
                     }
                     fence_proxy_async_smem();
                 }
@@ -312,11 +321,14 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         if (threadIdx.x == 0) paged_write_border(p, p.tile, p.start, worker, border, u_begin, range);
     } else if (warp == 4) {
         // =================== producer ======================================================
-        // lane (box, 64-channel block) looks up its piece of the next unit while this one is loaded, and
-        // issues that piece's copy
-        const int pieces = kPtBN / box_rows * KBQ;
-        const int box = lane / KBQ, kb = lane % KBQ;
-        const uint32_t at = kb * (kPtBN * 128) + box * box_rows * 128;
+        // lane (box, part of a head) looks up its piece of the next unit while this one is loaded, and
+        // issues that piece's copy of K; the first lane of a box also issues that of V
+        const int parts = k_whole ? 1 : KBQ;
+        const int pieces = kPtBN / box_rows * parts;
+        const int my_box = lane / parts, kb = lane % parts;
+        const uint32_t at_k = k_whole ? my_box * (KBQ * box_rows * 128)
+                                       : kb * (kPtBN * 128) + my_box * box_rows * 128;
+        const uint32_t at_v = my_box * (KBQ * box_rows * 128);
         int tile = tile0 - 1, j_next = 0, j_end = 0;
         bool have = true;                               // there is a next unit
         PagedTile t, nt = p.tile[tile0];
@@ -334,8 +346,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 n_first = p.start[tile + 1];            // long before it is needed
                 if (tile + 1 < tiles) nt = p.tile[tile + 1];
             }
-            next_col = t.kvh * D + kb * 64;
-            const int key = j_next * kPtBN + box * box_rows;
+            next_col = t.kvh * KBQ + kb;
+            const int key = j_next * kPtBN + my_box * box_rows;
             ++j_next;
             if (lane >= pieces || key >= t.kv_end) return;
             const int w = key / p.page;
@@ -365,7 +377,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 if (!__all_sync(0xffffffffu, ok)) break;
                 if (lane == 0) mbar_arrive_expect_tx(&k_full[s], L::kKV);
                 __syncwarp();
-                if (lane < pieces) tma_load_3d(sK + s * L::kKV + at, &tmK, &k_full[s], k_col, k_row, k_page);
+                if (lane < pieces) tma_load_4d(sK + s * L::kKV + at_k, &tmK, &k_full[s], 0, k_row, k_col, k_page);
             }
             if (j > 0) {
                 const int s = (j - 1) & 1;
@@ -374,7 +386,8 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                 if (!__all_sync(0xffffffffu, ok)) break;
                 if (lane == 0) mbar_arrive_expect_tx(&v_full[s], L::kKV);
                 __syncwarp();
-                if (lane < pieces) tma_load_3d(sV + s * L::kKV + at, &tmV, &v_full[s], v_col, v_row, v_page);
+                if (lane < pieces && kb == 0)
+                    tma_load_4d(sV + s * L::kKV + at_v, &tmV, &v_full[s], 0, v_row, v_col, v_page);
             }
             v_page = k_page;
             v_row = k_row;
@@ -385,6 +398,15 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         if (lane == 0) {
             const uint32_t idesc_s = umma_idesc_f16(kBf16 ? 1 : 0, kPtBM, kPtBN);
             const uint32_t idesc_o = umma_idesc_f16(kBf16 ? 1 : 0, kPtBM, D) | (1u << 16);   // B is MN-major
+            // distance of a head's 64-channel blocks of K; 8-row groups are 1024 bytes apart, but KBQ times
+            // that in boxes of 8 rows that hold whole heads (the descriptors' stride, in 16 bytes)
+            const uint32_t k_block = (k_whole ? box_rows : kPtBN) * 128;
+            const uint64_t spread = static_cast<uint64_t>((KBQ - 1) * 1024 >> 4) << 32;
+            const uint64_t k_spread = k_whole && box_rows == 8 ? spread : 0, v_spread = box_rows == 8 ? spread : 0;
+            uint32_t v_step[kPtBN / 16];                // where every 16th row of V is
+#pragma unroll
+            for (int k = 0; k < kPtBN / 16; ++k)
+                v_step[k] = (k * 16 / box_rows * KBQ * box_rows + k * 16 % box_rows) * 128;
             bool ok = true;
             int it = 0, seg = 0;
             int n_first = p.start[tile0], n_end = p.tile[tile0].kv_end;
@@ -400,7 +422,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
 #pragma unroll
                     for (int kb = 0; kb < KBQ; ++kb) {
                         const uint64_t a = umma_desc_k_sw128(smem_u32(sQ) + kb * (kPtBM * 128));
-                        const uint64_t b = umma_desc_k_sw128(smem_u32(sK) + s * L::kKV + kb * (kPtBN * 128));
+                        const uint64_t b = umma_desc_k_sw128(smem_u32(sK) + s * L::kKV + kb * k_block) + k_spread;
 #pragma unroll
                         for (int k = 0; k < 4; ++k)
                             umma_f16_ss(tmem_base + s * kPtBN, a + 2 * k, b + 2 * k, idesc_s, (kb | k) != 0 ? 1u : 0u);
@@ -419,7 +441,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                     tc_fence_after_sync();
 #pragma unroll
                     for (int k = 0; k < kPtBN / 16; ++k) {
-                        const uint64_t b = umma_desc_mn_sw128(smem_u32(sV) + s * L::kKV + k * 2048, kPtBN * 128);
+                        const uint64_t b = umma_desc_mn_sw128(smem_u32(sV) + s * L::kKV + v_step[k], box_rows * 128) + v_spread;
                         umma_f16_ts(tmem_o, tmem_base + s * kPtBN + k * 8, b, idesc_o, (j | k) != 0 ? 1u : 0u);
                     }
                     umma_commit(&pv_done[s]);
@@ -441,21 +463,28 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     }
 }
 
+template <int D, bool kBf16, int kBox>
+static int launch_tc_box(const PagedParams& p, int used, int box, cudaStream_t s)
+{
+    const bool k_whole = D == 64 || box == 8 || box == 64;
+    CUtensorMap tmK, tmV;
+    const uint64_t cols = static_cast<uint64_t>(p.Hk) * D;
+    int rc = make_tmap_paged_sw128(&tmK, p.K, cols, p.page, p.P, p.token_stride, p.page_stride, box, k_whole ? D / 64 : 1);
+    if (rc) return rc;
+    rc = make_tmap_paged_sw128(&tmV, p.V, cols, p.page, p.P, p.token_stride, p.page_stride, box, D / 64);
+    if (rc) return rc;
+    constexpr int smem = PtSmem<D>::kTotal;
+    DPK_CUDA(cudaFuncSetAttribute(paged_tc_kernel<D, kBf16, kBox>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    DPK_CUDA(paged_launch(paged_tc_kernel<D, kBf16, kBox>, dim3(used), kPtThreads, smem, s, tmK, tmV, p, box, k_whole));
+    return DPK_OK;
+}
+
 template <int D, bool kBf16>
 static int launch_tc(const PagedParams& p, int used, cudaStream_t s)
 {
     int box = 64;                                       // gcd(page, 64): page is a multiple of 8
     while (p.page % box) box >>= 1;
-    CUtensorMap tmK, tmV;
-    const uint64_t cols = static_cast<uint64_t>(p.Hk) * D;
-    int rc = make_tmap_3d_sw128(&tmK, p.K, cols, p.page, p.P, p.token_stride, p.page_stride, 64, box);
-    if (rc) return rc;
-    rc = make_tmap_3d_sw128(&tmV, p.V, cols, p.page, p.P, p.token_stride, p.page_stride, 64, box);
-    if (rc) return rc;
-    constexpr int smem = PtSmem<D>::kTotal;
-    DPK_CUDA(cudaFuncSetAttribute(paged_tc_kernel<D, kBf16>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    DPK_CUDA(paged_launch(paged_tc_kernel<D, kBf16>, dim3(used), kPtThreads, smem, s, tmK, tmV, p, box));
-    return DPK_OK;
+    return box == 64 ? launch_tc_box<D, kBf16, 64>(p, used, box, s) : launch_tc_box<D, kBf16, 0>(p, used, box, s);
 }
 
 int attn_paged_tc(const PagedParams& p, int D, int dtype, int used, cudaStream_t s)

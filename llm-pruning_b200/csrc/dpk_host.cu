@@ -89,6 +89,32 @@ int make_tmap_3d_sw128(CUtensorMap* map, const void* base, uint64_t cols, uint64
     return DPK_OK;
 }
 
+int make_tmap_paged_sw128(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t pages,
+                          uint64_t row_stride_elems, uint64_t page_stride_elems, uint32_t box_rows,
+                          uint32_t box_blocks)
+{
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return fail(DPK_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    if (!aligned16(base) || (row_stride_elems * 2) % 16 != 0 || (page_stride_elems * 2) % 16 != 0)
+        return fail(DPK_ERR_INVALID, "tensor base, row stride and page stride must be 16-byte aligned");
+    if (cols % 64 != 0 || box_rows == 0 || box_rows > 256 || box_blocks == 0 || box_blocks > cols / 64)
+        return fail(DPK_ERR_INVALID, "tensor-map box of %u rows and %u blocks out of range", box_rows, box_blocks);
+    if (pages == 0) pages = 1;
+    if (pages == 1) page_stride_elems = rows * row_stride_elems;      // unused, but must be valid
+    cuuint64_t dims[4] = {64, rows, cols / 64, pages};
+    cuuint64_t strides[3] = {row_stride_elems * 2, 128, page_stride_elems * 2};
+    cuuint32_t box[4] = {64, box_rows, box_blocks, 1};
+    cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void*>(base), dims, strides,
+                    box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail(DPK_ERR_CUDA,
+                    "cuTensorMapEncodeTiled (paged) failed with code %d (cols=%llu rows=%llu pages=%llu)",
+                    (int)r, (unsigned long long)cols, (unsigned long long)rows, (unsigned long long)pages);
+    return DPK_OK;
+}
+
 int make_tmap_2d_sw128(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows,
                        uint64_t row_stride_elems, uint32_t box_cols, uint32_t box_rows)
 {

@@ -41,6 +41,13 @@ int make_tmap_3d_sw128(CUtensorMap* map, const void* base, uint64_t cols, uint64
                        uint64_t batches, uint64_t row_stride_elems, uint64_t batch_stride_elems,
                        uint32_t box_cols, uint32_t box_rows);
 
+// Paged form: `pages` such 2-D tensors of `rows` rows, `page_stride_elems` apart, whose columns are counted
+// in blocks of 64: a 4-D map (64 columns, row, block, page) whose box is box_rows rows of box_blocks
+// blocks and lands in shared memory block by block (box_blocks x box_rows x 128 bytes).
+int make_tmap_paged_sw128(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t pages,
+                          uint64_t row_stride_elems, uint64_t page_stride_elems, uint32_t box_rows,
+                          uint32_t box_blocks);
+
 // Same, without swizzle (rows of the box stored back to back).
 int make_tmap_2d_plain(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows,
                        uint64_t row_stride_elems, uint32_t box_cols, uint32_t box_rows);

@@ -191,6 +191,10 @@ ATTN = [
     ([130, 1, 33], [200, 513, 31], 64, 16, 2, 128, 2, FP), # eight per KV head
     ([257], [64], 8, 10, 2, 64, 5, BF),                    # five per KV head, groups across KV heads
     ([90], [20], 40, 4, 1, 128, 1, BF),                    # whole-token routing, pages of 40
+    ([70, 30], [150, 77], 32, 8, 2, 128, 2, BF),           # boxes of 32 rows
+    ([70, 30], [150, 77], 96, 8, 2, 128, 0, FP),           # boxes of 32 rows in pages of 96
+    ([70, 30], [150, 77], 8, 8, 2, 128, 2, FP),            # boxes of 8 rows
+    ([70, 30], [150, 77], 48, 8, 2, 128, 4, BF),           # boxes of 16 rows, three a page
 ]
 
 

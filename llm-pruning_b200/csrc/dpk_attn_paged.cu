@@ -722,7 +722,7 @@ template <int D, bool kBf16>
 static int launch_join(const PagedParams& p, int used, cudaStream_t s)
 {
     int zero = (p.N + 3) / 4;
-    const int cap = sm_count() * 4;
+    const int cap = sm_count() * 8;
     if (zero > cap) zero = cap;
     if (p.tile_rows <= 16)
         DPK_CUDA(paged_launch(paged_join_kernel<D, kBf16, 1>, dim3(used * 4 + zero), 128, 0, s, p, 4, used * 4));

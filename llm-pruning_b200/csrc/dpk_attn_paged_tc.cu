@@ -69,25 +69,15 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    paged_wait_previous();
     paged_let_next_start();
-    const int tiles = p.head->tiles, length = p.head->length, range = p.head->range;
-    const int worker = blockIdx.x;
-    if (static_cast<int64_t>(worker) * range >= length) {           // whole CTA: nothing allocated yet
-        if (threadIdx.x == 0) p.border[worker].last_worker = -1;
-        return;
-    }
     if ((smem_u32(smem) & 1023u) != 0u) {
-        if (threadIdx.x == 0) atomicCAS(p.status, 0, 1000 * DPK_KERNEL_ID + DPK_DEV_BAD_SMEM_BASE);
+        if (threadIdx.x == 0) {
+            atomicCAS(p.status, 0, 1000 * DPK_KERNEL_ID + DPK_DEV_BAD_SMEM_BASE);
+            p.border[blockIdx.x].last_worker = -1;
+        }
         return;
     }
-    const int u_begin = worker * range, u_end = min(length, u_begin + range);
-    const int tile0 = paged_find_tile(p, p.tile, p.start, tiles, u_begin);
-    if (tile0 >= tiles || p.start[tile0] >= u_end) {                // only places between tiles
-        if (threadIdx.x == 0) p.border[worker].last_worker = -1;
-        return;
-    }
-
+    // what needs nothing of the work list is done while that is still being made
     if (warp == 4 && lane == 0) {
         mbar_init(q_full, 128);
         for (int s = 0; s < 2; ++s) {
@@ -111,7 +101,18 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
     const uint32_t tmem_base = *tmem_slot;
     const uint32_t tmem_o = tmem_base + 128;
 
-    if (warp < 4) {
+    paged_wait_previous();
+    const int tiles = p.head->tiles, length = p.head->length, range = p.head->range;
+    const int worker = blockIdx.x;
+    int u_begin = 0, u_end = 0, tile0 = tiles;
+    if (static_cast<int64_t>(worker) * range < length) {
+        u_begin = worker * range;
+        u_end = min(length, u_begin + range);
+        tile0 = paged_find_tile(p, p.tile, p.start, tiles, u_begin);
+    }
+    if (tile0 >= tiles || p.start[tile0] >= u_end) {    // nothing, or only places between tiles
+        if (threadIdx.x == 0) p.border[worker].last_worker = -1;
+    } else if (warp < 4) {
         // =================== softmax / epilogue: thread = row of the tile ==================
         const int row = warp * 32 + lane;
         const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;

@@ -159,7 +159,7 @@ def attention_paged(Q: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tenso
     Qc, q_ts = _token_rows(Q)
     clear = 0
     if O is None:
-        O = torch.empty_like(Q, memory_format=torch.contiguous_format)
+        O = torch.empty_like(Q) if Q.is_contiguous() else Q.new_empty((n, Hq, D))
         clear = 1
     elif O.shape != Q.shape or O.dtype != Q.dtype or not O.is_contiguous():
         raise ValueError("O must be contiguous with the shape and dtype of Q")
@@ -235,7 +235,7 @@ def _rope(dev, q, k, v, positions, inv_freq, sections, axis_map, interleaved, at
             kc, vc = k.contiguous(), v.contiguous()
             kv_ts = Hk * D
     if q_out is None:
-        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        q_out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((n, Hq, D))
         qo_ts = Hq * D
     else:
         if q_out.shape != q.shape or q_out.dtype != q.dtype:
@@ -245,7 +245,7 @@ def _rope(dev, q, k, v, positions, inv_freq, sections, axis_map, interleaved, at
             raise ValueError("q_out: the heads of a token must be contiguous, 16-byte aligned")
     k_out = None
     if cache is None:
-        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+        k_out = k.new_empty((n, Hk, D))
         tail = (None, None, 0, 0, None, 0, None, None, n, 0, 0, 0, 0)
     else:
         k_pages, v_pages, page_table, kv_lens, query_start = cache

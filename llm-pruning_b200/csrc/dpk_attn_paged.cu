@@ -17,7 +17,7 @@
 // rows behind the last key are zero-filled, so whatever an unused row of a page holds is never
 // multiplied).  It is bounded by HBM: 4 * D bytes per key against 16 MMA rows.
 #define DPK_KERNEL_ID 13   // thousands digit of the device status word
-#include "dpk_attn_paged.cuh"
+#include "dpk_attn_paged_plan.cuh"
 
 #include <math.h>
 
@@ -27,82 +27,6 @@ namespace dpk {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanItems = 4096;        // (sequence, KV head) pairs whose tile numbers fit shared memory
-
-// Sum over the block's threads, for two values at once; `sh` holds 32 pairs.  Every thread gets the
-// totals and the sums of the threads before it.
-__device__ __forceinline__ int2 plan_scan(int2 v, int2* sh, int2& total)
-{
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    int2 x = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x.x, o), z = __shfl_up_sync(0xffffffffu, x.y, o);
-        if (lane >= o) { x.x += y; x.y += z; }
-    }
-    __syncthreads();                       // the previous use of sh is over
-    if (lane == 31) sh[warp] = x;
-    __syncthreads();
-    if (warp == 0) {
-        int2 w = lane < warps ? sh[lane] : make_int2(0, 0);
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, w.x, o), z = __shfl_up_sync(0xffffffffu, w.y, o);
-            if (lane >= o) { w.x += y; w.y += z; }
-        }
-        sh[lane] = w;
-    }
-    __syncthreads();
-    total = sh[warps - 1];
-    const int2 before = warp ? sh[warp - 1] : make_int2(0, 0);
-    return make_int2(x.x - v.x + before.x, x.y - v.y + before.y);
-}
-
-// New tokens of sequence s, 0 where query_start does not make sense.
-__device__ __forceinline__ int plan_new(const PagedParams& p, int s, int& tok0)
-{
-    tok0 = p.qstart[s];
-    const int end = p.qstart[s + 1];
-    if (tok0 < 0 || end < tok0 || end > p.N) {
-        atomicCAS(p.status, 0, 1000 * DPK_KERNEL_ID + DPK_DEV_BAD_INDEX);
-        tok0 = 0;
-        return 0;
-    }
-    return end - tok0;
-}
-
-// Tile number `at` of an item of `rows` rows, and the units of its visible range.
-__device__ __forceinline__ int plan_tile(const PagedParams& p, int seq, int kvh, int at, int rows, PagedTile& t)
-{
-    t.seq = seq;
-    t.kvh = kvh;
-    const int fresh = plan_new(p, seq, t.tok0);
-    t.m0 = at * p.tile_rows;
-    t.rows = min(p.tile_rows, rows - t.m0);
-    t.kv_len = p.kv_lens[seq];
-    if (t.kv_len < 0 || t.kv_len > static_cast<int64_t>(p.W) * p.page) {
-        atomicCAS(p.status, 0, 1000 * DPK_KERNEL_ID + DPK_DEV_BAD_INDEX);
-        t.kv_len = 0;
-    }
-    t.pos0 = t.kv_len - fresh;
-    t.kv_end = t.kv_len;
-    int last = 0, head;
-    if (p.rows || !p.mask) {
-        if (p.causal) last = paged_row(p, t, t.rows - 1, head);
-    } else {                                     // the last row that is not routed out
-        last = -1;
-        for (int r = t.rows - 1; r >= 0 && last < 0; --r) last = paged_row(p, t, r, head);
-    }
-    if (p.causal) t.kv_end = min(t.kv_len, t.pos0 + last + 1);
-    return last >= 0 && t.kv_end > 0 ? paged_units(p, t) : 0;
-}
-
-// Where the tiles of (s, kvh) are put down by paged_rows_kernel: room for as many as its rows can need.
-__device__ __forceinline__ int plan_slot(const PagedParams& p, int s, int kvh)
-{
-    int tok0;
-    const int fresh = plan_new(p, s, tok0);
-    return p.Hk * (tok0 * p.rep / p.tile_rows + s) + kvh * (fresh * p.rep / p.tile_rows + 1);
-}
 
 // Active rows of every (sequence, KV head), in token order, and its tiles; used where tiles have many rows, so that
 // none of them is spent on a routed-out (token, head).  A thread looks at 16 rows in a row.
@@ -152,81 +76,6 @@ __global__ void __launch_bounds__(1024) paged_rows_kernel(const PagedParams p)
         if (plan_tile(p, s, kvh, t, carry, pt) == 0) pt.kv_end = 0;
         slot[t] = pt;
     }
-}
-
-// The whole block cuts the work: `tile`, `start` [tiles + 1] and `first` [S * Hk] may be shared memory.
-__device__ __forceinline__ void plan_work(const PagedParams& p, PagedTile* tile, int32_t* start, int* first,
-                                          int2* sh, int& tiles_out, int& length_out)
-{
-    const int tid = threadIdx.x, threads = blockDim.x;
-    const int items = p.S * p.Hk;
-    // 1. tiles of every (sequence, KV head)
-    int carry = 0;
-    for (int x0 = 0; x0 < items; x0 += threads) {
-        const int x = x0 + tid;
-        int n = 0;
-        if (x < items) {
-            int tok0;
-            const int rows = p.rows ? p.row_count[x] : plan_new(p, x / p.Hk, tok0) * p.rep;
-            n = (rows + p.tile_rows - 1) / p.tile_rows;
-        }
-        int2 t;
-        const int2 at = plan_scan(make_int2(n, 0), sh, t);
-        if (x < items) first[x] = carry + at.x;
-        carry += t.x;
-    }
-    const int tiles = min(carry, p.max_tiles);
-    __syncthreads();
-    // 2. the visible keys of every tile; tiles without any are dropped.  Worker after worker gets every
-    //    workers-th tile, so that tiles that are worked on at the same time are neighbours and read the same
-    //    K and V: in order, each worker would keep to its own sequences, and together they would go
-    //    through more K and V than L2 holds (12 sequences of 509 tokens over 3000, 64 heads: 739 us
-    //    instead of 837; where it all fits L2 the order makes no difference).
-    //    Worker g's share of the T tiles is every place of the line in [g T / W, (g + 1) T / W), so that all
-    //    workers pass their k-th tile at about the same time.
-    const int rounds = tiles / p.workers;            // tiles that every worker has; some have one more
-    int kept = 0, length = 0;
-    for (int q0 = 0; q0 < tiles; q0 += threads) {
-        const int q = q0 + tid;
-        int n = 0;
-        PagedTile pt = {};
-        if (q < tiles) {
-            // max_tiles * workers < 2^31 was checked
-            const int g = ((q + 1) * p.workers - 1) / tiles, g_first = g * tiles / p.workers, k = q - g_first;
-            const int t = k < rounds ? k * p.workers + g : rounds * p.workers + g_first - g * rounds;
-            int lo = 0, hi = items - 1;
-            while (lo < hi) {                        // last item that starts at or before t
-                const int mid = (lo + hi + 1) >> 1;
-                if (first[mid] <= t) lo = mid;
-                else hi = mid - 1;
-            }
-            const int s = lo / p.Hk, kvh = lo - s * p.Hk;
-            if (p.rows) {
-                pt = p.slot[plan_slot(p, s, kvh) + t - first[lo]];
-                n = paged_units(p, pt);
-            } else {
-                int tok0;
-                n = plan_tile(p, s, kvh, t - first[lo], plan_new(p, s, tok0) * p.rep, pt);
-            }
-        }
-        int2 total;
-        const int2 at = plan_scan(make_int2(n > 0, n > 0 ? n + p.tile_gap : 0), sh, total);
-        if (n > 0) {
-            tile[kept + at.x] = pt;
-            start[kept + at.x] = length + at.y;
-        }
-        kept += total.x;
-        length += total.y;
-    }
-    if (tid == 0) start[kept] = length;
-    __syncthreads();
-    tiles_out = kept;
-    length_out = length;
-}
-
-__device__ __forceinline__ int plan_range(const PagedParams& p, int length)
-{
-    return max((length + p.workers - 1) / p.workers, p.min_range);
 }
 
 __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedParams p)
@@ -289,8 +138,9 @@ __device__ __forceinline__ uint32_t pw_off(int r, int c)
 
 // Up to kPwTiles tiles (a decode step of 16 sequences with 8 KV heads) the attention kernel makes the work
 // list itself, every CTA for its own use in shared memory behind the rings: that saves a launch of a
-// kernel that takes as long as a small step's attention (8 tiles: 22 us a call instead of 27).  A
-// CTA of 128 threads takes longer over a long list than the launch does (512 tiles: 262 us instead of 258).
+// kernel that takes as long as a small step's attention (8 tiles: 11.4 us on the device instead of 12.5,
+// 22.7 a call instead of 26.2).  A CTA of 128 threads takes longer over a long list than the launch does
+// (128 tiles: the same on the device; 512: 262 us instead of 258).
 constexpr int kPwTiles = 144;
 
 template <int D, bool kBf16, bool kPlanHere>
@@ -530,8 +380,8 @@ __global__ void __launch_bounds__(kPwWarps * 32) paged_warp_kernel(const PagedPa
 
 // The last join_blocks = workers * row_groups blocks join the tiles that several workers shared: block
 // (w, g) takes a share of the rows of the tile that starts in worker w's range and ends behind it.
-// Where that are up to eight parts a warp joins kRows rows by itself, their loads in flight
-// together; else the block's four warps share the parts of each row.  The blocks before write the
+// Few parts: a warp joins kRows rows by itself, their loads in flight together; many parts of few
+// rows: the block's four warps share the parts of each row.  The blocks before write the
 // rows that no unit covers, a token per warp: routed out, without a visible key, and (clear_tail)
 // behind the last sequence.  They need nothing of the attention kernel, so they do not wait for it.
 struct JoinRow {
@@ -583,7 +433,12 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p, in
             for (int c = 0; c < C; c += 2)
                 *reinterpret_cast<uint32_t*>(out + c * 2) = pack_half2<kBf16>(acc[c] * inv, acc[c + 1] * inv);
         };
-        if (w1 - w0 < 8) {
+        // steps of either way: a warp takes kRows rows and two parts at a time, a block a row and 16 parts
+        // and a barrier
+        const int parts = w1 - w0 + 1, at_once = row_groups * 4 * kRows;
+        const int by_warp = (t.rows + at_once - 1) / at_once * ((parts + 1) / 2);
+        const int by_block = (t.rows + row_groups - 1) / row_groups * ((parts + 15) / 16 + 1);
+        if (by_warp <= by_block) {
             for (int r = (group * 4 + warp) * kRows; r < t.rows; r += row_groups * 4 * kRows) {
                 int i[kRows], head[kRows];
                 JoinRow s[kRows];
@@ -753,7 +608,8 @@ static PagedShape paged_shape(int64_t N, int S, int Hq, int Hk, int D, int max_q
     g.tile_gap = g.tc ? 3 : 1;
     g.min_range = 2;
     g.max_tiles = int64_t(Hk) * ((N * rep) / g.tile_rows + S);
-    g.plan_here = !g.tc && g.max_tiles <= kPwTiles && int64_t(S) * Hk <= kPwTiles;
+    const int here = g.tc ? kPtTiles : kPwTiles;
+    g.plan_here = g.max_tiles <= here && int64_t(S) * Hk <= here;
     size_t at = 16;
     auto take = [&](size_t bytes) {
         const size_t here = at;
@@ -875,12 +731,12 @@ int dpk_attn_paged(const void* Q, const void* K, const void* V, const int32_t* p
         const int threads = per_thread >= 1024 ? 1024 : static_cast<int>((per_thread + 31) / 32 * 32);
         paged_rows_kernel<<<dim3(S, Hk), threads, 0, s>>>(p);
         DPK_CUDA(cudaGetLastError());
-        DPK_CUDA(paged_launch(paged_plan_kernel, dim3(1), plan_threads, 0, s, p));
+        if (!g.plan_here) DPK_CUDA(paged_launch(paged_plan_kernel, dim3(1), plan_threads, 0, s, p));
     } else if (!g.plan_here) {
         paged_plan_kernel<<<1, plan_threads, 0, s>>>(p);
         DPK_CUDA(cudaGetLastError());
     }
-    const int rc = g.tc ? attn_paged_tc(p, D, dtype, static_cast<int>(used), s)
+    const int rc = g.tc ? attn_paged_tc(p, D, dtype, static_cast<int>(used), g.plan_here, s)
                         : attn_paged_warp(p, D, dtype, static_cast<int>(used), g.plan_here, s);
     if (rc) return rc;
     if (D == 64) return dtype == DPK_BF16 ? launch_join<64, true>(p, (int)used, s) : launch_join<64, false>(p, (int)used, s);

@@ -77,6 +77,7 @@ __device__ __forceinline__ int paged_row(const PagedParams& p, const PagedTile& 
 {
     int x = t.m0 + r;
     head = t.kvh * p.rep;
+    if (x < 0) return -1;
     if (p.rows) {
         const int64_t at = static_cast<int64_t>(t.tok0) * p.rep + x;
         if (at >= static_cast<int64_t>(p.N) * p.rep) return -1;
@@ -154,6 +155,9 @@ __device__ __forceinline__ float paged_exp2(float x)
 }
 
 // `used`: workers that can get work
-int attn_paged_tc(const PagedParams& p, int D, int dtype, int used, cudaStream_t s);
+int attn_paged_tc(const PagedParams& p, int D, int dtype, int used, bool plan_here, cudaStream_t s);
+
+// Tiles up to which the chunk kernel makes the work list itself (see dpk_attn_paged_tc.cu).
+constexpr int kPtTiles = 256;
 
 }  // namespace dpk

@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(kPlanThreads) paged_plan_kernel(const PagedPar
     if (threadIdx.x == 0) {
         p.head->tiles = tiles;
         p.head->length = length;
-        p.head->range = plan_range(p, length);
+        p.head->range = plan_range(p, tiles, length);
     }
 }
 
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(kPwWarps * 32) paged_warp_kernel(const PagedPa
         tile_of = reinterpret_cast<PagedTile*>(smem + kPwWarps * WARP_B);
         start = reinterpret_cast<int32_t*>(tile_of + kPwTiles);
         plan_work(p, tile_of, start, start + kPwTiles + 1, sh, tiles, length);
-        range = plan_range(p, length);
+        range = plan_range(p, tiles, length);
     } else {
         paged_wait_previous();
         tiles = p.head->tiles;

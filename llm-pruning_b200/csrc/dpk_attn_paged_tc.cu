@@ -114,7 +114,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         PagedTile* my_tiles = reinterpret_cast<PagedTile*>(smem + L::kOffPlan);
         int32_t* my_start = reinterpret_cast<int32_t*>(my_tiles + kPtTiles);
         plan_work(p, my_tiles, my_start, my_start + kPtTiles + 1, sh, tiles, length);
-        range = plan_range(p, length);
+        range = plan_range(p, tiles, length);
         tile_of = my_tiles;
         start = my_start;
     } else {

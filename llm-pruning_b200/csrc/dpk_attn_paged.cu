@@ -623,7 +623,7 @@ static PagedShape paged_shape(int64_t N, int S, int Hq, int Hk, int D, int max_q
     g.off_rows = take(g.tc && has_mask ? size_t(Hk) * N * rep * 4 : 0);
     g.off_count = take(g.tc && has_mask ? size_t(S) * Hk * 4 : 0);
     g.off_border = take(size_t(g.workers) * sizeof(PagedBorder));
-    g.off_o = take(size_t(g.workers) * 2 * g.tile_rows * D * 4);
+    g.off_o = take(size_t(g.workers) * 2 * g.tile_rows * D * 4 + 16);      // room to start on 32 bytes
     g.off_ml = take(size_t(g.workers) * 2 * g.tile_rows * 8);
     g.bytes = at;
     return g;
@@ -712,7 +712,7 @@ int dpk_attn_paged(const void* Q, const void* K, const void* V, const int32_t* p
     p.rows = g.tc && mask ? reinterpret_cast<int32_t*>(w + g.off_rows) : nullptr;
     p.row_count = g.tc && mask ? reinterpret_cast<int32_t*>(w + g.off_count) : nullptr;
     p.border = reinterpret_cast<PagedBorder*>(w + g.off_border);
-    p.part_o = reinterpret_cast<float*>(w + g.off_o);
+    p.part_o = reinterpret_cast<float*>((reinterpret_cast<uintptr_t>(w + g.off_o) + 31) & ~uintptr_t(31));
     p.part_ml = reinterpret_cast<float*>(w + g.off_ml);
     p.tile_rows = g.tile_rows; p.unit_keys = g.unit_keys; p.tile_gap = g.tile_gap;
     p.workers = workers; p.min_range = g.min_range;

@@ -43,6 +43,15 @@ struct PtSmem {
     static constexpr int kTotalPlan = kOffPlan + kPtTiles * (int(sizeof(PagedTile)) + 8) + 4;
 };
 
+// 32 bytes, a whole sector, from one thread (32-byte aligned): a warp's rows lie far apart, and 16-byte stores
+// would send each sector twice.
+__device__ __forceinline__ void pt_store_sector(void* dst, const uint32_t (&w)[8])
+{
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(w[0]), "r"(w[1]),
+                 "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+
 // kBox: rows of a box where that is known at compile time (64: one box a unit), else 0.
 template <int D, bool kBf16, int kBox>
 __global__ void __launch_bounds__(kPtThreads, 2)
@@ -135,6 +144,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
         // =================== softmax / epilogue: thread = row of the tile ==================
         const int row = warp * 32 + lane;
         const uint32_t lane_base = static_cast<uint32_t>(warp * 32) << 16;
+        const bool o_sectors = (reinterpret_cast<uintptr_t>(p.O) & 31u) == 0;
         bool alive = true;
         int it = 0;                                     // units done, over all tiles
         int border = -1;
@@ -312,20 +322,28 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
                     if (tok < 0) continue;
                     if (whole) {
 #pragma unroll
-                        for (int q4 = 0; q4 < 4; ++q4) {
-                            uint32_t w[4];
+                        for (int q2 = 0; q2 < 2; ++q2) {
+                            uint32_t w[8];
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                w[i] = pack_half2<kBf16>(__uint_as_float(v[q4 * 8 + 2 * i]) * inv,
-                                                         __uint_as_float(v[q4 * 8 + 2 * i + 1]) * inv);
-                            *reinterpret_cast<uint4*>(out + (c + q4 * 8) * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+                            for (int i = 0; i < 8; ++i)
+                                w[i] = pack_half2<kBf16>(__uint_as_float(v[q2 * 16 + 2 * i]) * inv,
+                                                         __uint_as_float(v[q2 * 16 + 2 * i + 1]) * inv);
+                            if (o_sectors) {
+                                pt_store_sector(out + (c + q2 * 16) * 2, w);
+                            } else {
+                                uint4* dst = reinterpret_cast<uint4*>(out + (c + q2 * 16) * 2);
+                                dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                                dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+                            }
                         }
                     } else {
                         float* dst = p.part_o + slot * D + c;
 #pragma unroll
-                        for (int q4 = 0; q4 < 8; ++q4)
-                            *reinterpret_cast<uint4*>(dst + q4 * 4) =
-                                make_uint4(v[q4 * 4], v[q4 * 4 + 1], v[q4 * 4 + 2], v[q4 * 4 + 3]);
+                        for (int q = 0; q < 4; ++q) {
+                            const uint32_t w[8] = {v[q * 8], v[q * 8 + 1], v[q * 8 + 2], v[q * 8 + 3],
+                                                   v[q * 8 + 4], v[q * 8 + 5], v[q * 8 + 6], v[q * 8 + 7]};
+                            pt_store_sector(dst + q * 8, w);
+                        }
                     }
                 }
                 if (!whole && tok >= 0) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(m_ref, l_sum);

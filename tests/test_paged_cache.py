@@ -284,6 +284,11 @@ def test_attention_paged_strides(ops, most):
     got, _ = ops.attention_paged(q, token_major[:, :, 0], token_major[:, :, 1], wide[:, 5:5 + W], d["lens"],
                                  d["start"], max_query_len=most)
     assert torch.equal(got, want)
+    room = torch.zeros(36 * 8 * 128 + 8, dtype=BF, device="cuda")          # an output that starts on 16 bytes
+    mine = room[8:].view(36, 8, 128)
+    got, _ = ops.attention_paged(q, pool[:, 0], pool[:, 1], wide[:, 5:5 + W], d["lens"], d["start"], O=mine,
+                                 max_query_len=most)
+    assert got is mine and torch.equal(mine, want) and (room[:8] == 0).all()
     check_attention(want, b)
 
 

@@ -234,8 +234,7 @@ __global__ void __launch_bounds__(kPwWarps * 32) paged_warp_kernel(const PagedPa
         int head0 = 0, head1 = 0;
         const int i0 = gid < t.rows ? paged_row(p, t, gid, head0) : -1;
         const int i1 = gid + 8 < t.rows ? paged_row(p, t, gid + 8, head1) : -1;
-        const int lim0 = i0 < 0 ? -1 : p.causal ? min(t.kv_len - 1, t.pos0 + i0) : t.kv_len - 1;
-        const int lim1 = i1 < 0 ? -1 : p.causal ? min(t.kv_len - 1, t.pos0 + i1) : t.kv_len - 1;
+        const int lim0 = paged_last_key(p, t, i0), lim1 = paged_last_key(p, t, i1);
         uint32_t qf[KS][4];
         {
             const uint8_t* q0 = p.Q + ((t.tok0 + max(i0, 0)) * p.q_ts + static_cast<int64_t>(head0) * D) * 2 + t4 * 4;
@@ -345,7 +344,7 @@ __global__ void __launch_bounds__(kPwWarps * 32) paged_warp_kernel(const PagedPa
         l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
         l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
         if (j1 - j0 == t_units) {                            // the whole tile was this warp's
-            const float inv0 = l0 > 0.f ? 1.f / l0 : 0.f, inv1 = l1 > 0.f ? 1.f / l1 : 0.f;
+            const float inv0 = paged_inverse(lim0, l0), inv1 = paged_inverse(lim1, l1);
             uint8_t* d0 = p.O + ((static_cast<int64_t>(t.tok0 + max(i0, 0)) * p.Hq + head0) * D + 2 * t4) * 2;
             uint8_t* d1 = p.O + ((static_cast<int64_t>(t.tok0 + max(i1, 0)) * p.Hq + head1) * D + 2 * t4) * 2;
 #pragma unroll
@@ -391,7 +390,7 @@ struct JoinRow {
 template <int C>
 __device__ __forceinline__ void join_add(JoinRow& s, float (&acc)[C], const float2& ml, const float (&x)[C], float scale_log2)
 {
-    if (ml.x == -INFINITY) return;
+    if (ml.y == 0.f) return;               // no weight in this part; a sum that is NaN stays in, whatever its maximum
     const float top = fmaxf(s.m, ml.x);
     const float a = paged_exp2((s.m - top) * scale_log2), b = paged_exp2((ml.x - top) * scale_log2);
     s.l = s.l * a + ml.y * b;
@@ -427,7 +426,7 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p, in
         if (w1 < 0) return;
         auto slot_of = [&](int w, int r) { return (static_cast<int64_t>(w) * 2 + (w == w0 ? slot0 : 0)) * p.tile_rows + r; };
         auto store = [&](int i, int head, const JoinRow& s, const float (&acc)[C]) {
-            const float inv = s.l > 0.f ? 1.f / s.l : 0.f;
+            const float inv = paged_inverse(paged_last_key(p, t, i), s.l);
             uint8_t* out = p.O + ((static_cast<int64_t>(t.tok0 + i) * p.Hq + head) * D + lane * C) * 2;
 #pragma unroll
             for (int c = 0; c < C; c += 2)

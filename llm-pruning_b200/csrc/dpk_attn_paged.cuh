@@ -90,6 +90,17 @@ __device__ __forceinline__ int paged_row(const PagedParams& p, const PagedTile& 
     return i;
 }
 
+// Last key that new token i of the tile's sequence sees, -1 or less where it sees none (or i is -1: no row).
+__device__ __forceinline__ int paged_last_key(const PagedParams& p, const PagedTile& t, int i)
+{
+    return i < 0 ? -1 : p.causal ? min(t.kv_len - 1, t.pos0 + i) : t.kv_len - 1;
+}
+
+// What a row's sum of weighted values is multiplied by.  A row that sees no key is zero; any other is divided by the
+// sum of its weights whatever that is: NaN where a score it sees is NaN or +inf, 0 (and so 0 * inf, NaN) where all
+// its scores are -inf -- the softmax of such rows has no value, and the row says so, however the work was cut.
+__device__ __forceinline__ float paged_inverse(int last_key, float l) { return last_key < 0 ? 0.f : 1.f / l; }
+
 __device__ __forceinline__ int paged_units(const PagedParams& p, const PagedTile& t)
 {
     return (t.kv_end + p.unit_keys - 1) / p.unit_keys;

@@ -184,7 +184,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             const int n_first = start[tile + 1];           // what the next tile needs, long before
             more = tile + 1 < tiles && n_first < u_end;
             if (more) nt = tile_of[tile + 1];
-            const int lim = tok < 0 ? -1 : p.causal ? min(t.kv_len - 1, t.pos0 + tok) : t.kv_len - 1;
+            const int lim = paged_last_key(p, t, tok);
             // the fewest keys that a row of the warp sees: its first row's (rows are in token order)
             const int lim_first = __shfl_sync(0xffffffffu, lim, 0);
             const bool idle = warp * 32 >= t.rows;      // none of this warp's rows exists
@@ -311,7 +311,7 @@ paged_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__
             tc_fence_after_sync();
             if (!idle) {
                 const bool whole = j1 - j0 == t_units;
-                const float inv = l_sum > 0.f ? 1.f / l_sum : 0.f;
+                const float inv = paged_inverse(lim, l_sum);
                 const int64_t slot = (static_cast<int64_t>(worker) * 2 + (t_first > u_begin ? 1 : 0)) * kPtBM + row;
                 uint8_t* out = p.O + (static_cast<int64_t>(t.tok0 + max(tok, 0)) * p.Hq + head) * (D * 2);
 #pragma unroll 1

@@ -1,0 +1,124 @@
+"""The paged-cache operators at the edges of what a call may hold: values that are no numbers, starts that make no
+sense, sequences that got no room, counts that disagree with tables, tensors off their alignment, empty states,
+buffers of captured steps, the rarer dispatch paths and pools beyond 2^31 elements.
+
+Tolerances are those of ``test_paged_cache`` (64-bit and integer oracles, roundings counted per element)."""
+
+import math
+
+import pytest
+import torch
+
+from oracle import paged_oracle as PO
+from test_paged_cache import BF, FP, Cache, check_attention, check_rotated, cuda, make, rope_case, u_of
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from dpk_b200 import build, ops
+    build.build()
+    return ops
+
+
+@pytest.fixture(autouse=True)
+def _status_clean(request, ops):
+    yield
+    if torch.cuda.is_available() and "gpu" in request.keywords:
+        assert ops.device_status() == 0
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def poison(like, value):
+    """Leaves ``value`` in memory that the allocator hands out again for tensors of this size."""
+    held = [torch.full_like(like, value) for _ in range(4)]
+    torch.cuda.synchronize()
+    del held
+
+
+# ------------------------------------------------------------------ values that are no numbers (GPU)
+
+def check_not_numbers(got, b, mask=None, q=None):
+    """NaN exactly where the 64-bit form has it; the other rows within the bounds of ``check_attention``."""
+    q = b["q"] if q is None else q
+    want, size = PO.attention(q, b["k"], b["v"], b["table"], b["lens"], b["start"], mask)
+    got, lost = got.detach().cpu().double(), want.isnan()
+    assert torch.equal(got.isnan(), lost)
+    u = u_of(b["q"].dtype)
+    tol = u * want.abs() + (u + 2.0 ** -13) * size + 2.0 ** -25
+    assert ((got - want).abs() <= tol)[~lost].all()
+    return lost
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("most", [1, 64])
+@pytest.mark.parametrize("cached", [20, 40000])      # a tile of one worker; a part of it with every worker
+def test_attention_paged_nan_query(ops, cached, most):
+    b = make([3], [cached], 32, 8, 2, 64, BF, seed=41)
+    mask = torch.ones(3, 8, dtype=torch.bool)
+    mask[2, 3] = False
+    clean = b["q"].clone()
+    clean[1, 5] = math.nan
+    b["q"][1, 5] = b["q"][2, 3] = math.nan           # the second one is routed out
+    d = cuda(b)
+    got, _ = ops.attention_paged(d["q"], d["k"], d["v"], d["table"], d["lens"], d["start"], mask.cuda(),
+                                 max_query_len=most)
+    lost = check_not_numbers(got, b, mask, clean)
+    assert lost[1, 5].all() and int(lost.sum()) == 64 and (got[2, 3] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("most", [1, 64])
+@pytest.mark.parametrize("first,last", [(0, 6000), (17000, 17001), (12000, 40001)])
+def test_attention_paged_nan_keys(ops, first, last, most):
+    """A stretch of NaN keys over several workers' ranges, one key, and the keys up to the second token."""
+    b = make([4], [40000], 32, 8, 2, 64, BF, seed=42)
+    for pos in range(first, last):
+        b["k"][b["table"][0, pos // 32], pos % 32, 0] = math.nan
+    d = cuda(b)
+    got, _ = ops.attention_paged(d["q"], d["k"], d["v"], d["table"], d["lens"], d["start"], max_query_len=most)
+    lost = check_not_numbers(got, b)
+    assert lost[:, :4].all() and not lost[:, 4:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("most", [1, 64])
+def test_attention_paged_nan_keys_up_to_a_workers_border(ops, most):
+    """A stretch of NaN keys that ends after every unit in turn: with the first worker's range too."""
+    b = make([4], [40000], 32, 8, 2, 64, BF, seed=42)
+    d = cuda(b)
+    for unit in range(60):
+        d["k"][d["table"][0, unit].long(), :, 0] = math.nan
+        got, _ = ops.attention_paged(d["q"], d["k"], d["v"], d["table"], d["lens"], d["start"], max_query_len=most)
+        lost = got.isnan()
+        assert lost[:, :4].all() and not lost[:, 4:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("most", [1, 64])
+def test_attention_paged_nan_key_of_a_later_token(ops, most):
+    b = make([4, 2], [30, 0], 16, 8, 2, 128, FP, seed=43)
+    b["k"][b["table"][0, 32 // 16], 32 % 16, 1] = math.nan          # the third new token's
+    d = cuda(b)
+    got, _ = ops.attention_paged(d["q"], d["k"], d["v"], d["table"], d["lens"], d["start"], max_query_len=most)
+    lost = check_not_numbers(got, b)
+    assert lost[2:4, 4:].all() and int(lost.sum()) == 2 * 4 * 128
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("most", [1, 64])
+@pytest.mark.parametrize("cached", [20, 40000])
+def test_attention_paged_infinite_scores(ops, cached, most):
+    """Scores of -inf alone leave no weights (NaN); beside a finite one they weigh nothing; +inf is NaN."""
+    b = make([2], [cached], 32, 6, 3, 64, BF, seed=44)
+    b["q"] = b["q"].abs() + 0.25
+    b["k"][:, :, 0] = -math.inf
+    b["k"][:, :, 1] = -math.inf
+    b["k"][b["table"][0, 0], 5, 1] = 0.5
+    b["k"][b["table"][0, 0], 7, 2] = math.inf
+    d = cuda(b)
+    got, _ = ops.attention_paged(d["q"], d["k"], d["v"], d["table"], d["lens"], d["start"], max_query_len=most)
+    lost = check_not_numbers(got, b)
+    assert lost[:, :2].all() and not lost[:, 2:4].any() and lost[:, 4:].all()

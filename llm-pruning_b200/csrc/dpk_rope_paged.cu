@@ -44,6 +44,11 @@ struct RopePagedParams {
     int* status;
 };
 
+__device__ __forceinline__ void rope_report(const RopePagedParams& p)
+{
+    atomicCAS(p.status, 0, 1000 * DPK_KERNEL_ID + DPK_DEV_BAD_INDEX);
+}
+
 template <bool kBf16>
 __device__ __forceinline__ void turn_half(uint4& a, uint4& b, const float2* cs)
 {
@@ -82,9 +87,11 @@ constexpr int kRopeFlight = 4;           // heads of a lane in flight
 // so the 8 angles it needs stay in registers; a warp covers 32 / (D/16) heads per step.  Nothing is
 // shared between warps: one warp's lookups and sines are hidden by the others' copies.  A CTA per
 // token with a barrier between angles and copies measured 130 to 157 us where this takes 114 (16384
-// tokens, 64 + 2 * 8 heads of 128: 5.9 TB/s; 2 heads in flight 117, 8 heads 128).
+// tokens, 64 + 2 * 8 heads of 128: 5.9 TB/s; 2 heads in flight 117, 8 heads 128).  The bound of five CTAs per SM
+// holds the kernel at 96 registers; with the 111 it takes otherwise four fit, and those 16384 tokens take 117 us instead
+// of 113 replayed from a graph.
 template <bool kBf16, bool kNear>
-__global__ void __launch_bounds__(kRopeWarps * 32) rope_paged_kernel(const RopePagedParams p, int split)
+__global__ void __launch_bounds__(kRopeWarps * 32, 5) rope_paged_kernel(const RopePagedParams p, int split)
 {
     __shared__ float2 sh_cs[kRopeWarps][kRopeMaxPairs];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -109,11 +116,16 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_paged_kernel(const RopeP
                 hi = min(hi, lo + n * width);
                 lo += (n - 1) * width;
             }
-            const int pos = p.kv_lens[lo] - p.qstart[lo + 1] + t;
+            // The place follows from the end of the sequence's new tokens, so a start that makes no sense would name
+            // tokens that are cached already: only a sequence whose range is one has places.
+            const int begin = p.qstart[lo], end = p.qstart[lo + 1], len = p.kv_lens[lo];
+            const bool sound = begin >= 0 && begin <= t && t < end && end <= p.N &&
+                               len <= static_cast<int64_t>(p.W) * p.page;
+            const int pos = len - end + t;
             const int w = pos / p.page;
-            const int id = pos >= 0 && w < p.W ? p.table[lo * p.table_stride + w] : -1;
+            const int id = sound && pos >= 0 && w < p.W ? p.table[lo * p.table_stride + w] : -1;
             if (id >= 0 && id < p.P) row = id * p.page_stride + (pos - w * p.page) * p.token_stride;
-            else if (lane == 0) atomicCAS(p.status, 0, 1000 * DPK_KERNEL_ID + DPK_DEV_BAD_INDEX);   // q is turned all the same
+            else if (lane == 0) rope_report(p);          // q is turned all the same
         }
         __syncwarp();
         for (int i = lane; i < p.R / 2; i += 32) {
@@ -121,7 +133,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_paged_kernel(const RopeP
             if (p.axis_map) {
                 axis = p.axis_map[i];
                 if (axis < 0 || axis >= p.axes) {
-                    atomicCAS(p.status, 0, 1000 * DPK_KERNEL_ID + DPK_DEV_BAD_INDEX);
+                    rope_report(p);
                     axis = 0;
                 }
             } else {
@@ -186,6 +198,14 @@ __global__ void __launch_bounds__(kRopeWarps * 32) rope_paged_kernel(const RopeP
                     *reinterpret_cast<uint4*>(dst + hi_at) = hi[k];
                 }
             }
+        }
+    }
+    // starts that no token looked at: sequences without a row, a first start that is not 0
+    if (p.k_pages) {
+        const int64_t all = static_cast<int64_t>(gridDim.x) * (kRopeWarps * 32);
+        for (int64_t s = static_cast<int64_t>(blockIdx.x) * (kRopeWarps * 32) + threadIdx.x; s < p.S; s += all) {
+            const int begin = p.qstart[s], end = p.qstart[s + 1];
+            if (begin < 0 || end < begin || end > p.N || (s == 0 && begin != 0)) rope_report(p);
         }
     }
 }

@@ -122,3 +122,53 @@ def test_attention_paged_infinite_scores(ops, cached, most):
     got, _ = ops.attention_paged(d["q"], d["k"], d["v"], d["table"], d["lens"], d["start"], max_query_len=most)
     lost = check_not_numbers(got, b)
     assert lost[:, :2].all() and not lost[:, 2:4].any() and lost[:, 4:].all()
+
+
+# ------------------------------------------------------------------ starts that make no sense (GPU)
+
+STARTS = [
+    # starts, rows of q
+    ([0, 5], 1),                # one sequence that ends behind the tensors
+    ([2, 3, 5], 5),             # tokens before the first sequence
+    ([-3, 2, 4], 4),
+    ([0, 2, 9], 4),
+    ([0, 4, 99], 4),            # the second sequence has no row at all
+    ([0, 5, 3, 8], 8),          # backwards, and two sequences that overlap
+    ([0, -1], 2),
+    ([6, 2, 4], 6),
+]
+
+
+def owned(start, n):
+    """Tokens that a sequence whose range makes sense names."""
+    return {t for a, b in zip(start, start[1:]) if 0 <= a <= b <= n for t in range(a, b)}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", range(len(STARTS)))
+def test_rope_append_paged_bad_starts(ops, case):
+    """Only the new tokens' places of sequences whose range makes sense are written, and the status says so."""
+    start, n = STARTS[case]
+    S, page, D = len(start) - 1, 8, 64
+    lens = [20 + 3 * s for s in range(S)]
+    b = make([0] * S, lens, page, 2, 2, D, BF, seed=45)
+    g = b["gen"]
+    q, k, v = (torch.randn(n, 2, D, generator=g).to(BF) for _ in range(3))
+    pos = torch.arange(n)[None]
+    inv = torch.ones(D // 2)
+    d = cuda(b)
+    dk, dv, dpos = k.cuda(), v.cuda(), pos.cuda()
+    ops.rope_append_paged(q.cuda(), dk, dv, dpos, inv.cuda(), d["k"], d["v"], d["table"], d["lens"], i32(start))
+    assert ops.device_status() == 15105
+    kr = ops.rope_axes(q.cuda(), dk, dpos, inv.cuda())[1].cpu()
+    free = torch.zeros(b["k"].shape[:2], dtype=torch.bool)
+    for s, (a, e) in enumerate(zip(start, start[1:])):
+        if not 0 <= a <= e <= n:
+            continue
+        for t in range(a, e):
+            at = lens[s] - (e - t)
+            place = (int(b["table"][s, at // page]), at % page)
+            free[place] = True
+            if sum(x <= t < y for x, y in zip(start, start[1:]) if 0 <= x <= y <= n) == 1 and start == sorted(start):
+                assert torch.equal(d["k"][place].cpu(), kr[t]) and torch.equal(d["v"][place].cpu(), v[t])
+    assert torch.equal(d["k"].cpu()[~free], b["k"][~free]) and torch.equal(d["v"].cpu()[~free], b["v"][~free])

@@ -365,9 +365,10 @@ int dpk_rope_append(void* q, void* k, const void* v, const void* cos, const void
  *   kv_lens    [S]    int32   tokens of a sequence in the cache, the new ones of a step included
  *   ref_counts [P]    int32   number of sequences that hold a page, 0 = free
  *   query_start [S+1] int32   first new token of each sequence in Q / q / k / v; [0] = 0, [S] = the end
- * The host never reads any of it.  A page id, length or index outside its range is reported in the
+ * The host never reads any of it.  A page id, length or start outside its range is reported in the
  * status word (code 105; kernel 13 attention on warps, 14 attention on tensor-memory tiles, 15
- * rotary embedding, 16 pages) and never followed.  No reference counterpart: the reference's cache
+ * rotary embedding, 16 pages) and never followed; a sequence whose range of tokens runs backwards or
+ * leaves [0, N] has none, and rows before query_start[0] belong to no sequence.  No reference counterpart: the reference's cache
  * is contiguous (WIDE/wrapper/cache.py:10-60).
  */
 
@@ -378,8 +379,8 @@ int dpk_rope_append(void* q, void* k, const void* v, const void* cos, const void
  *   Q [N,Hq,D] (q_token_stride), K, V [P,page_size,Hk,D] (page_stride, page_token_stride; K and V
  *   alike), mask [N,NG] bytes or NULL = every head, O [N,Hq,D] packed.  Strides in elements,
  *   multiples of 8; 0 = packed.
- * Rows of O of routed-out heads and of tokens that see no key are zero; rows behind
- * query_start[S] are left as they are, or zeroed with clear_tail.  What the cache holds behind
+ * Rows of O of routed-out heads and of tokens that see no key are zero; rows of no sequence (behind
+ * query_start[S]) are left as they are, or zeroed with clear_tail.  What the cache holds behind
  * kv_lens, in pages no sequence holds, or in keys that a token may not see, has no influence (values
  * that a token may not see but another new token of its sequence may: finite values only).
  * max_query_len: an upper bound of n_s.  It chooses the kernel and the size of the workspace; a

@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(kPwWarps * 32) paged_warp_kernel(const PagedPa
 // Few parts: a warp joins kRows rows by itself, their loads in flight together; many parts of few
 // rows: the block's four warps share the parts of each row.  The blocks before write the
 // rows that no unit covers, a token per warp: routed out, without a visible key, and (clear_tail)
-// behind the last sequence.  They need nothing of the attention kernel, so they do not wait for it.
+// of no sequence.  They need nothing of the attention kernel, so they do not wait for it.
 struct JoinRow {
     float m, l;
 };
@@ -507,10 +507,9 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p, in
         return;
     }
     for (int t = blockIdx.x * 4 + warp; t < p.N; t += zero_blocks * 4) {
-        const bool tail = p.S == 0 || t >= p.qstart[p.S];
-        if (tail && !p.clear_tail) continue;
         int seen = -1;                                       // last key the token sees
-        if (!tail) {
+        bool owned = false;                                  // some sequence's token
+        if (p.S > 0 && t < p.qstart[p.S]) {
             int lo = 0, hi = p.S;                            // last sequence that starts at or before t
             while (hi - lo > 1) {
                 const int step = (hi - lo + 31) / 32;
@@ -520,9 +519,14 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p, in
                 hi = min(hi, lo + n * step);
                 lo = lo + (n - 1) * step;
             }
-            const int len = p.kv_lens[lo];
+            const int begin = p.qstart[lo], end = p.qstart[lo + 1], len = p.kv_lens[lo];
+            owned = begin >= 0 && begin <= t && t < end && end <= p.N;       // those that plan_new accepts
             seen = len <= 0 || len > static_cast<int64_t>(p.W) * p.page ? -1
-                   : p.causal ? min(len - 1, len - p.qstart[lo + 1] + t) : len - 1;
+                   : p.causal ? min(len - 1, len - end + t) : len - 1;
+        }
+        if (!owned) {                                        // behind the last sequence, or a start makes no sense
+            if (!p.clear_tail) continue;
+            seen = -1;
         }
         if (seen >= 0 && !p.mask) continue;
         constexpr int kLanes = D / 8, kAtOnce = 32 / kLanes;     // lanes of a head's row, rows of a store

@@ -45,6 +45,8 @@ __device__ __forceinline__ int plan_new(const PagedParams& p, int s, int& tok0)
         tok0 = 0;
         return 0;
     }
+    if (s == 0 && tok0 != 0)               // rows before the first sequence belong to none, like those behind the last
+        atomicCAS(p.status, 0, 1000 * DPK_KERNEL_ID + DPK_DEV_BAD_INDEX);
     return end - tok0;
 }
 

@@ -7,7 +7,8 @@ current stream, ``ValueError`` for refused arguments, nothing read back to the h
 State of a cache (int32 tensors on the GPU): ``page_table [S,W]`` page ids, ``kv_lens [S]`` tokens
 held (a step's new ones included), ``ref_counts [P]`` holders of a page, 0 = free.  A step names its
 new tokens by ``query_start [S+1]``: those of sequence ``s`` are rows ``query_start[s] ..
-query_start[s+1]-1`` of the packed q/k/v.  :class:`dpk_b200.wide.PagedKVCache` keeps the state.
+query_start[s+1]-1`` of the packed q/k/v; the first start is 0, and a sequence whose range is none (it
+runs backwards or leaves the tensors) is reported and has no tokens.  :class:`dpk_b200.wide.PagedKVCache` keeps the state.
 No reference counterpart (its cache is contiguous, ``WIDE/wrapper/cache.py:10-60``); values outside
 their range are reported through :func:`dpk_b200.ops.device_status` and never followed.
 """
@@ -126,8 +127,8 @@ def attention_paged(Q: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tenso
     [P,page_size,Hk,D]`` already hold them (:func:`rope_append_paged`).  New token ``i`` of the ``n``
     new ones of sequence ``s`` sees keys ``j <= kv_lens[s] - n + i``, or with ``is_causal=False`` all
     ``kv_lens[s]`` of them.  ``Mask [N,NG]`` (non-zero = active) routes head groups as everywhere
-    else; ``None`` keeps every head.  Rows that are routed out or see no key are zero.  Rows behind
-    ``query_start[S]`` are zero in a new ``O`` and left alone in one that is passed in.
+    else; ``None`` keeps every head.  Rows that are routed out or see no key are zero.  Rows of no
+    sequence (behind ``query_start[S]``) are zero in a new ``O`` and left alone in one that is passed in.
 
     ``max_query_len``: an upper bound of a sequence's new tokens, known to the host (default: N).
     It chooses between the kernel for a few tokens per sequence and the one for chunks, so give 1

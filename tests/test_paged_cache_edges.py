@@ -172,3 +172,29 @@ def test_rope_append_paged_bad_starts(ops, case):
             if sum(x <= t < y for x, y in zip(start, start[1:]) if 0 <= x <= y <= n) == 1 and start == sorted(start):
                 assert torch.equal(d["k"][place].cpu(), kr[t]) and torch.equal(d["v"][place].cpu(), v[t])
     assert torch.equal(d["k"].cpu()[~free], b["k"][~free]) and torch.equal(d["v"].cpu()[~free], b["v"][~free])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("most", [1, 64])
+@pytest.mark.parametrize("case", range(len(STARTS)))
+def test_attention_paged_bad_starts(ops, case, most, masked):
+    """Rows that no sequence names are zero in a new output and left alone in a given one."""
+    start, n = STARTS[case]
+    S = len(start) - 1
+    b = make([0] * S, [20 + 3 * s for s in range(S)], 8, 4, 2, 64, BF, seed=46)
+    q = torch.randn(n, 4, 64, generator=b["gen"]).to(BF).cuda()
+    mask = torch.ones(n, 2, dtype=torch.bool, device="cuda") if masked else None
+    d = cuda(b)
+    other = [t for t in range(n) if t not in owned(start, n)]
+    poison(q, 7.0)
+    got, _ = ops.attention_paged(q, d["k"], d["v"], d["table"], d["lens"], i32(start), mask, max_query_len=most)
+    assert ops.device_status() % 1000 == 105
+    assert (got[other] == 0).all() and torch.isfinite(got).all() and not (got == 7).any()
+    mine = torch.full_like(q, 7.0)
+    ops.attention_paged(q, d["k"], d["v"], d["table"], d["lens"], i32(start), mask, O=mine, max_query_len=most)
+    assert ops.device_status() % 1000 == 105
+    assert (mine[other] == 7).all()
+    if start == sorted(start):
+        mine[other] = 0
+        assert torch.equal(mine, got)

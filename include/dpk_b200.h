@@ -421,6 +421,22 @@ int dpk_rope_append_paged(const void* q, const void* k, const void* v, void* q_o
                           int Hq, int Hk, int D, int dtype, void* stream);
 
 /*
+ * The same for a step whose tokens are sent whether or not there was room for them (a captured one):
+ * `granted` [S] is what dpk_page_extend left for this step, 0 = refused.  The length of a refused
+ * sequence does not count its new tokens, so their places would be cached tokens': with `granted` their
+ * k and v are written nowhere and nothing is reported, their q is turned like any other.  NULL: all granted.
+ */
+int dpk_rope_append_paged_granted(const void* q, const void* k, const void* v, void* q_out, void* k_out,
+                                  int64_t q_token_stride, int64_t kv_token_stride, int64_t q_out_token_stride,
+                                  const void* positions, int64_t axis_stride, int positions_64,
+                                  const float* inv_freq, const int32_t* axis_map, const int32_t* sections,
+                                  int axes, int rotary, int neighbours, float scale, void* k_pages,
+                                  void* v_pages, int64_t page_stride, int64_t page_token_stride,
+                                  const int32_t* page_table, int64_t table_stride, const int32_t* kv_lens,
+                                  const int32_t* query_start, int N, int S, int W, int P, int page_size,
+                                  int Hq, int Hk, int D, int dtype, const uint8_t* granted, void* stream);
+
+/*
  * Pages: bookkeeping on the device, and the bytes it makes move, in every layer of both pools.
  * Pools: k, v [layers, P, page_size * row_elems] (layer_stride, page_stride in elements, a page
  * contiguous).  Workspace: dpk_page_workspace_bytes(S or 0, P or 0, n or 0).

@@ -37,6 +37,7 @@ struct RopePagedParams {
     const int32_t* table;    // [S, W]
     const int32_t* kv_lens;  // [S]
     const int32_t* qstart;   // [S + 1]
+    const uint8_t* granted;  // [S] or NULL: 0 where the cache had no room for the new tokens
     int64_t q_ts, kv_ts, qo_ts, page_stride, token_stride, table_stride, axis_stride;   // elements
     int ends[kRopeMaxAxes];  // axis a serves the pairs below ends[a] that no earlier axis serves
     float scale;             // of cos and sin
@@ -121,11 +122,13 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 5) rope_paged_kernel(const Ro
             const int begin = p.qstart[lo], end = p.qstart[lo + 1], len = p.kv_lens[lo];
             const bool sound = begin >= 0 && begin <= t && t < end && end <= p.N &&
                                len <= static_cast<int64_t>(p.W) * p.page;
+            // a refused sequence's length does not count its new tokens: the place would be a cached token's
+            const bool refused = sound && p.granted && p.granted[lo] == 0;
             const int pos = len - end + t;
             const int w = pos / p.page;
-            const int id = sound && pos >= 0 && w < p.W ? p.table[lo * p.table_stride + w] : -1;
+            const int id = sound && !refused && pos >= 0 && w < p.W ? p.table[lo * p.table_stride + w] : -1;
             if (id >= 0 && id < p.P) row = id * p.page_stride + (pos - w * p.page) * p.token_stride;
-            else if (lane == 0) rope_report(p);          // q is turned all the same
+            else if (lane == 0 && !refused) rope_report(p);      // q is turned all the same
         }
         __syncwarp();
         for (int i = lane; i < p.R / 2; i += 32) {
@@ -229,15 +232,33 @@ static void launch_rope(const RopePagedParams& p, cudaStream_t s)
 
 using namespace dpk;
 
-extern "C" int dpk_rope_append_paged(const void* q, const void* k, const void* v, void* q_out, void* k_out,
-                                     int64_t q_token_stride, int64_t kv_token_stride, int64_t q_out_token_stride,
-                                     const void* positions, int64_t axis_stride, int positions_64,
-                                     const float* inv_freq, const int32_t* axis_map, const int32_t* sections,
-                                     int axes, int rotary, int neighbours, float scale, void* k_pages,
-                                     void* v_pages, int64_t page_stride, int64_t page_token_stride,
-                                     const int32_t* table, int64_t table_stride, const int32_t* kv_lens,
-                                     const int32_t* query_start, int N, int S, int W, int P, int page_size,
-                                     int Hq, int Hk, int D, int dtype, void* stream)
+extern "C" {
+
+int dpk_rope_append_paged(const void* q, const void* k, const void* v, void* q_out, void* k_out,
+                          int64_t q_token_stride, int64_t kv_token_stride, int64_t q_out_token_stride,
+                          const void* positions, int64_t axis_stride, int positions_64, const float* inv_freq,
+                          const int32_t* axis_map, const int32_t* sections, int axes, int rotary, int neighbours,
+                          float scale, void* k_pages, void* v_pages, int64_t page_stride, int64_t page_token_stride,
+                          const int32_t* table, int64_t table_stride, const int32_t* kv_lens,
+                          const int32_t* query_start, int N, int S, int W, int P, int page_size, int Hq, int Hk,
+                          int D, int dtype, void* stream)
+{
+    return dpk_rope_append_paged_granted(q, k, v, q_out, k_out, q_token_stride, kv_token_stride, q_out_token_stride,
+                                         positions, axis_stride, positions_64, inv_freq, axis_map, sections, axes,
+                                         rotary, neighbours, scale, k_pages, v_pages, page_stride, page_token_stride,
+                                         table, table_stride, kv_lens, query_start, N, S, W, P, page_size, Hq, Hk, D,
+                                         dtype, nullptr, stream);
+}
+
+int dpk_rope_append_paged_granted(const void* q, const void* k, const void* v, void* q_out, void* k_out,
+                                  int64_t q_token_stride, int64_t kv_token_stride, int64_t q_out_token_stride,
+                                  const void* positions, int64_t axis_stride, int positions_64,
+                                  const float* inv_freq, const int32_t* axis_map, const int32_t* sections, int axes,
+                                  int rotary, int neighbours, float scale, void* k_pages, void* v_pages,
+                                  int64_t page_stride, int64_t page_token_stride, const int32_t* table,
+                                  int64_t table_stride, const int32_t* kv_lens, const int32_t* query_start, int N,
+                                  int S, int W, int P, int page_size, int Hq, int Hk, int D, int dtype,
+                                  const uint8_t* granted, void* stream)
 {
     DPK_REQUIRE(q && k && q_out && positions && inv_freq, "NULL tensor");
     DPK_REQUIRE((k_pages == nullptr) == (v_pages == nullptr), "k_pages and v_pages go together");
@@ -290,6 +311,7 @@ extern "C" int dpk_rope_append_paged(const void* q, const void* k, const void* v
     p.table = table;
     p.kv_lens = kv_lens;
     p.qstart = query_start;
+    p.granted = granted;
     p.q_ts = q_token_stride;
     p.kv_ts = kv_token_stride;
     p.qo_ts = q_out_token_stride;
@@ -314,3 +336,5 @@ extern "C" int dpk_rope_append_paged(const void* q, const void* k, const void* v
     DPK_CUDA(cudaGetLastError());
     return DPK_OK;
 }
+
+}  // extern "C"

@@ -64,6 +64,9 @@ SIGNATURES = {
     "dpk_rope_append_paged": (_i32, [_vp] * 5 + [_i64] * 3 + [_vp, _i64, _i32, _vp, _vp, _vp, _i32, _i32,
                                      _i32, _f32, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _vp]
                               + [_i32] * 9 + [_vp]),
+    "dpk_rope_append_paged_granted": (_i32, [_vp] * 5 + [_i64] * 3 + [_vp, _i64, _i32, _vp, _vp, _vp, _i32, _i32,
+                                             _i32, _f32, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _vp]
+                                      + [_i32] * 9 + [_vp, _vp]),
     "dpk_page_workspace_bytes": (_sz, [_i32, _i32, _i32]),
     "dpk_page_extend": (_i32, [_vp, _i64, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i32,
                                _i64, _i64, _i32, _vp, _sz, _vp]),

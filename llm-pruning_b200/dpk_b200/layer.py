@@ -159,8 +159,9 @@ class RoutedDecoderLayer:
         (:class:`dpk_b200.wide.PagedKVCache`, its ``extend`` called for this step): prompt chunks, single
         tokens and drafts side by side.  ``x [N,H]``, the new tokens back to back (``query_start``);
         ``positions [axes,N]`` or ``[N]`` and ``inv_freq`` as :func:`ops.rope_append_paged` takes them, with
-        its ``sections`` / ``axis_map`` / ``interleaved`` / ``attention_scale``; ``layer``: this layer's
-        number in the cache."""
+        its ``sections`` / ``axis_map`` / ``interleaved`` / ``attention_scale`` / ``granted``; ``layer``: this
+        layer's number in the cache.  Tokens of a row that the cache refused may be sent: they change
+        nothing in it."""
         f = self.front
         N = x.shape[0]
         x3 = x[None]

@@ -193,7 +193,8 @@ def _host_ints(values: tuple):
     return (ctypes.c_int32 * len(values))(*values)
 
 
-def _rope(dev, q, k, v, positions, inv_freq, sections, axis_map, interleaved, attention_scale, q_out, cache):
+def _rope(dev, q, k, v, positions, inv_freq, sections, axis_map, interleaved, attention_scale, q_out, cache,
+          granted=None):
     code = _code(q)
     if k.dtype != q.dtype or (v is not None and v.dtype != q.dtype):
         raise ValueError("q, k and v must share one dtype")
@@ -258,18 +259,22 @@ def _rope(dev, q, k, v, positions, inv_freq, sections, axis_map, interleaved, at
         S, W, tstride = _table(page_table)
         _ints(kv_lens, (S,), "kv_lens")
         _ints(query_start, (S + 1,), "query_start")
+        if granted is not None and (granted.dtype not in (torch.bool, torch.uint8) or granted.shape != (S,)
+                                    or not granted.is_contiguous()):
+            raise ValueError(f"granted must be a contiguous bool or uint8 tensor of shape [{S}], got "
+                             f"{granted.dtype} {list(granted.shape)}")
         if S == 0:
             return q_out, None
         tail = (k_pages.data_ptr(), v_pages.data_ptr(), ps, ts, page_table.data_ptr(), tstride,
                 kv_lens.data_ptr(), query_start.data_ptr(), n, S, W, P, page)
     if n == 0:
         return q_out, k_out
-    _call(dev, N.load().dpk_rope_append_paged,
+    _call(dev, N.load().dpk_rope_append_paged_granted,
           qc.data_ptr(), kc.data_ptr(), None if vc is None else vc.data_ptr(), q_out.data_ptr(),
           None if k_out is None else k_out.data_ptr(), q_ts, kv_ts, qo_ts, positions.data_ptr(), axis_stride,
           1 if positions.dtype is torch.int64 else 0, inv_freq.data_ptr(),
           None if axis_map is None else axis_map.data_ptr(), secs, axes, rotary, 1 if interleaved else 0,
-          float(attention_scale), *tail, Hq, Hk, D, code)
+          float(attention_scale), *tail, Hq, Hk, D, code, None if granted is None else granted.data_ptr())
     return q_out, k_out
 
 
@@ -278,7 +283,8 @@ def rope_append_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positio
                       page_table: torch.Tensor, kv_lens: torch.Tensor, query_start: torch.Tensor,
                       sections: Optional[Sequence[int]] = None, axis_map: Optional[torch.Tensor] = None,
                       interleaved: bool = False, attention_scale: float = 1.0,
-                      q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                      q_out: Optional[torch.Tensor] = None,
+                      granted: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Rotary embedding with one or several position axes, and the write of the rotated ``k`` and of
     ``v`` into the pages of the new tokens; returns the rotated ``q [N,Hq,D]`` (in ``q_out``, which
     may be ``q`` itself).
@@ -292,10 +298,15 @@ def rope_append_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positio
     and sin.  A token's place in the cache is its place in the sequence (the last tokens of
     ``kv_lens[s]``), whatever its rotary positions.  Rows behind ``query_start[S]`` are not touched (in a
     new ``q`` they hold anything).  Counterpart of :func:`rope_append`; computed
-    from positions, so far ones keep their exact angle."""
-    dev = _on_gpu(q, k, v, positions, inv_freq, K_pages, V_pages, page_table, kv_lens, query_start, axis_map, q_out)
+    from positions, so far ones keep their exact angle.
+
+    ``granted [S]`` (bool or uint8): what :func:`page_extend` returned for this step.  A refused sequence's
+    length does not count its new tokens, so they have no place: with ``granted`` their ``k`` and ``v`` are
+    left out, without it such a sequence must bring none."""
+    dev = _on_gpu(q, k, v, positions, inv_freq, K_pages, V_pages, page_table, kv_lens, query_start, axis_map, q_out,
+                  granted)
     return _rope(dev, q, k, v, positions, inv_freq, sections, axis_map, interleaved, attention_scale, q_out,
-                 (K_pages, V_pages, page_table, kv_lens, query_start))[0]
+                 (K_pages, V_pages, page_table, kv_lens, query_start), granted)[0]
 
 
 def rope_axes(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor,
@@ -366,7 +377,8 @@ def page_extend(K_pages: torch.Tensor, V_pages: torch.Tensor, page_table: torch.
     the sequences in row order), writes them into ``page_table`` and adds to ``kv_lens``.  A partly
     filled last page that other sequences hold too is copied, in all layers, before it is written to
     (where all its holders write, the first keeps it).  Returns ``granted [S]`` bool; a sequence that
-    is not granted -- the free pages or its row of the table do not suffice -- is left as it was."""
+    is not granted -- the free pages or its row of the table do not suffice -- is left as it was, and
+    has no places for its new tokens: see ``granted`` of :func:`rope_append_paged`."""
     dev = _on_gpu(page_table, kv_lens, ref_counts, add, K_pages, V_pages)
     st = _state(page_table, kv_lens, ref_counts)
     pools, P, page = _pools(K_pages, V_pages)

@@ -200,13 +200,14 @@ class PagedKVCache:
     GPU and is never read back, so a whole serving step can be captured into a graph:
 
     * ``page_table [max_sequences, ceil(max_length / page_size)]`` int32, ``lengths [max_sequences]`` int32,
-      ``ref_counts [pages]`` int32;
+      ``ref_counts [pages]`` int32, ``granted [max_sequences]`` bool (of the last ``extend``);
     * ``keys, values [layers, pages, page_size, num_kv_heads, head_dim]``.
 
     A step: ``granted = cache.extend(add)``; per layer ``q = cache.rope_update(layer, q, k, v, ...)`` and
     ``o = cache.attend(layer, q, ...)`` with the new tokens of all sequences back to back, those of
-    row ``s`` at ``query_start[s] .. query_start[s+1]-1`` (as many as ``add[s]``; a row that was not granted
-    must bring none).  No reference counterpart (its cache is one contiguous tensor per layer,
+    row ``s`` at ``query_start[s] .. query_start[s+1]-1``, as many as ``add[s]``.  A row that was not granted
+    keeps its length and what it holds; its tokens may be sent all the same (those of a captured step are):
+    their keys and values are written nowhere, and their outputs are of no use.  No reference counterpart (its cache is one contiguous tensor per layer,
     ``WIDE/wrapper/cache.py:10-60``)."""
 
     def __init__(self, layers: int, pages: int, page_size: int, num_kv_heads: int, head_dim: int,
@@ -220,11 +221,14 @@ class PagedKVCache:
         self.page_table = torch.full((max_sequences, -(-max_length // page_size)), -1, **ints)
         self.lengths = torch.zeros(max_sequences, **ints)
         self.ref_counts = torch.zeros(pages, **ints)
+        self.granted = torch.ones(max_sequences, dtype=torch.bool, device=device)
         self.page_size = page_size
 
     def extend(self, add: torch.Tensor) -> torch.Tensor:
         """Room for ``add [max_sequences]`` more tokens; ``granted`` bool (:func:`ops.page_extend`)."""
-        return ops.page_extend(self.keys, self.values, self.page_table, self.lengths, self.ref_counts, add)
+        granted = ops.page_extend(self.keys, self.values, self.page_table, self.lengths, self.ref_counts, add)
+        self.granted.copy_(granted)          # a place of its own: captured writes read it at every replay
+        return granted
 
     def fork(self, parents: torch.Tensor, children: torch.Tensor) -> torch.Tensor:
         """Empty rows ``children`` share everything of rows ``parents`` (:func:`ops.page_fork`)."""
@@ -247,7 +251,8 @@ class PagedKVCache:
                     query_start: torch.Tensor, **kw) -> torch.Tensor:
         """Writes the rotated keys and the values of the new tokens into ``layer`` and returns the rotated
         queries (:func:`ops.rope_append_paged`; ``sections``, ``axis_map``, ``interleaved``,
-        ``attention_scale``, ``q_out`` pass through)."""
+        ``attention_scale``, ``q_out`` pass through; ``granted`` is the last ``extend``'s unless given)."""
+        kw.setdefault("granted", self.granted)
         return ops.rope_append_paged(query_states, key_states, value_states, positions, inv_freq, self.keys[layer],
                                      self.values[layer], self.page_table, self.lengths, query_start, **kw)
 

@@ -198,3 +198,91 @@ def test_attention_paged_bad_starts(ops, case, most, masked):
     if start == sorted(start):
         mine[other] = 0
         assert torch.equal(mine, got)
+
+
+# ------------------------------------------------------------------ sequences that got no room (GPU)
+
+@pytest.mark.gpu
+def test_rope_append_paged_leaves_refused_sequences_alone(ops):
+    b, near = rope_case(1)
+    d = cuda(b)
+    granted = torch.tensor([True, False, True], device="cuda")
+    q = ops.rope_append_paged(d["q"], d["kn"], d["vn"], d["pos"], d["inv"], d["k"], d["v"], d["table"], d["lens"],
+                              d["start"], sections=b["sections"], granted=granted)
+    check_rotated(q, b["q"], b, near)                 # the queries are turned all the same
+    kr = ops.rope_axes(d["q"], d["kn"], d["pos"], d["inv"], b["sections"])[1].cpu()
+    k, v = b["k"].clone(), b["v"].clone()
+    for s in (0, 2):
+        at = int(b["lens"][s]) - 1
+        place = (int(b["table"][s, at // 16]), at % 16)
+        k[place], v[place] = kr[s], b["vn"][s]
+    assert torch.equal(d["k"].cpu(), k) and torch.equal(d["v"].cpu(), v)
+    for bad in (granted.int(), granted[:2], granted.cpu()):
+        with pytest.raises(ValueError):
+            ops.rope_append_paged(d["q"], d["kn"], d["vn"], d["pos"], d["inv"], d["k"], d["v"], d["table"],
+                                  d["lens"], d["start"], sections=b["sections"], granted=bad)
+
+
+@pytest.mark.gpu
+def test_decode_step_in_one_graph_with_a_pool_that_runs_out(ops):
+    """A captured step brings a token for every row.  A refused row's tokens change nothing that is cached, not
+    in pages that it shares either, and it goes on where it stopped once there is room."""
+    from dpk_b200.wide import PagedKVCache
+
+    g = torch.Generator().manual_seed(52)
+    S, Hq, Hk, D, page = 4, 4, 2, 64, 8
+    cache = PagedKVCache(1, 6, page, Hk, D, S, 64, BF, "cuda")
+    add, start = i32([1] * S), i32(list(range(S + 1)))
+    q, k, v = (torch.zeros(S, h, D, dtype=BF, device="cuda") for h in (Hq, Hk, Hk))
+    inv = torch.ones(D // 2, device="cuda")
+
+    def step():
+        granted = cache.extend(add)
+        qr = cache.rope_update(0, q, k, v, cache.lengths[None], inv, start)
+        return granted, qr, cache.attend(0, qr, start, max_query_len=1)
+    step()
+    cache.free(i32(list(range(S))))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        granted, qr, out = step()
+    keys, values = [[] for _ in range(S)], [[] for _ in range(S)]
+    refused = 0
+
+    def replay():
+        nonlocal refused
+        for t in (q, k, v):
+            t.copy_(torch.randn(t.shape, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        lens, table, ok = cache.lengths.tolist(), cache.page_table.tolist(), granted.tolist()
+        kr = ops.rope_axes(q, k, cache.lengths[None], inv)[1].cpu()
+        for s in range(S):
+            if ok[s]:
+                keys[s].append(kr[s])
+                values[s].append(v[s].cpu())
+            refused += not ok[s]
+            assert lens[s] == len(keys[s])
+            for j in range(lens[s]):
+                place = (0, table[s][j // page], j % page)
+                assert torch.equal(cache.keys[place].cpu(), keys[s][j])
+                assert torch.equal(cache.values[place].cpu(), values[s][j])
+            if ok[s]:
+                one = dict(q=qr[s:s + 1].cpu(), k=torch.stack(keys[s])[None], v=torch.stack(values[s])[None],
+                           table=torch.zeros(1, 1, dtype=torch.int32), lens=torch.tensor([lens[s]]),
+                           start=torch.tensor([0, 1]))
+                check_attention(out[s:s + 1], one)
+
+    for _ in range(14):                               # 4 rows of pages of 8 in a pool of 6
+        replay()
+    assert refused >= 4
+    cache.free(i32([3]))                              # one page is free: row 2 takes it, and rows 0 and 3, which
+    assert cache.fork(i32([0]), i32([3])).all()       # share a partly filled page, cannot write to it
+    keys[3], values[3] = list(keys[0]), list(values[0])
+    for _ in range(2):
+        replay()
+        assert granted.tolist() == [False, True, True, False]
+    cache.free(i32([1]))
+    keys[1], values[1] = [], []
+    replay()
+    assert granted.tolist() == [True] * 4

@@ -454,7 +454,8 @@ int dpk_rope_append_paged_granted(const void* q, const void* k, const void* v, v
  * copy: page dst[i] becomes a copy of page src[i].  Of several pairs with one destination the last
  *   counts; a pair whose source is another pair's destination is left out and reported.
  * compact: moves the held pages into [0, live), each hole in ascending order taking the next held
- *   page behind `live`; rewrites table and ref_counts; live [1] int32 = their number.
+ *   page behind `live`; rewrites table and ref_counts; live [1] int32 = their number.  An entry of a
+ *   sequence's pages whose count is 0 is reported and becomes -1.
  */
 size_t dpk_page_workspace_bytes(int S, int P, int n);
 int dpk_page_extend(int32_t* page_table, int64_t table_stride, int32_t* kv_lens, int32_t* ref_counts,

@@ -415,6 +415,7 @@ page_compact_kernel(const PageState st, int32_t* __restrict__ remap, int32_t* __
     for (int c0 = p0; c0 < p1; c0 += kPgThreads) {
         const int p = c0 + tid;
         const bool used = p < p1 && st.refs[p] > 0;
+        if (p < p1 && !(used && p >= live)) remap[p] = used ? p : -1;      // the moved ones follow below
         const int is_hole = p < p1 && p < live && !used, is_mover = used && p >= live;
         int hk, mk;
         const int a = block_scan(is_hole, sh, hk);
@@ -439,19 +440,22 @@ page_compact_kernel(const PageState st, int32_t* __restrict__ remap, int32_t* __
     }
 }
 
+// An entry whose page nobody holds (counts and table disagree) would name another sequence's page from here
+// on, or one that is handed out next: it is reported and becomes -1, which no operator follows.
 __global__ void __launch_bounds__(256)
-page_remap_kernel(const PageState st, const int32_t* __restrict__ remap, const int32_t* __restrict__ live)
+page_remap_kernel(const PageState st, const int32_t* remap)
 {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int limit = *live;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
          i < static_cast<int64_t>(st.S) * st.W; i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
         const int s = static_cast<int>(i / st.W), w = static_cast<int>(i - static_cast<int64_t>(s) * st.W);
         if (w >= pages_of(st.lens[s], st.page)) continue;
         int32_t* e = st.table + s * st.table_stride + w;
-        if (*e < 0 || *e >= st.P) page_report(st.status);
-        else if (*e >= limit) *e = remap[*e];
+        const int id = *e;
+        const int to = id < 0 || id >= st.P ? -1 : remap[id];
+        if (to < 0) page_report(st.status);
+        if (to != id && id >= 0 && id < st.P) *e = to;
     }
 }
 
@@ -714,7 +718,7 @@ int dpk_page_compact(void* k, void* v, int layers, int64_t layer_stride, int64_t
     if (S > 0 && W > 0) {
         int64_t blocks = (static_cast<int64_t>(S) * W + 255) / 256;
         if (blocks > sm_count() * 8) blocks = sm_count() * 8;
-        rc = launch_early(blocks, page_remap_kernel, s, st, remap, live);
+        rc = launch_early(blocks, page_remap_kernel, s, st, remap);
         if (rc) return rc;
     }
     return move_pages(st, pp, P / 2 + 1, 40, s);

@@ -437,7 +437,7 @@ def page_compact(K_pages: torch.Tensor, V_pages: torch.Tensor, page_table: torch
                  kv_lens: torch.Tensor, ref_counts: torch.Tensor) -> torch.Tensor:
     """Moves the held pages to the front of the pools (each hole, in ascending order, takes the next
     held page behind), rewrites ``page_table`` and ``ref_counts``.  Returns their number, int32 ``[1]``:
-    pages from there on are free."""
+    pages from there on are free.  An entry whose page nobody holds by the counts is reported and becomes -1."""
     dev = _on_gpu(page_table, kv_lens, ref_counts, K_pages, V_pages)
     st = _state(page_table, kv_lens, ref_counts)
     pools, P, page = _pools(K_pages, V_pages)

@@ -286,3 +286,21 @@ def test_decode_step_in_one_graph_with_a_pool_that_runs_out(ops):
     keys[1], values[1] = [], []
     replay()
     assert granted.tolist() == [True] * 4
+
+
+# ------------------------------------------------------------------ counts that disagree (GPU)
+
+@pytest.mark.gpu
+def test_page_compact_reports_entries_of_pages_that_nobody_holds(ops):
+    from dpk_b200 import _native as N
+    c = Cache(4, 3, 8, 8)
+    c.extend(ops, [9, 3, 0, 0])                       # pages 0, 1 and 2
+    c.trim(ops, [0])                                  # page 2 is the only one left
+    c.table[2, 0], c.lens[2] = 6, 5                   # behind the pages that stay, held by nobody
+    c.table[3, 0], c.lens[3] = 0, 5                   # the hole that page 2 moves to
+    poison(torch.empty((N.load().dpk_page_workspace_bytes(0, 8, 0) + 3) // 4, dtype=torch.int32, device="cuda"), 3)
+    live = ops.page_compact(c.k, c.v, c.table, c.lens, c.refs)
+    assert ops.device_status() == 16105
+    assert live.tolist() == [1] and c.refs.tolist() == [1] + [0] * 7
+    assert c.table.tolist() == [[-1] * 3, [0, -1, -1], [-1] * 3, [-1] * 3]
+    assert torch.equal(c.k[:, 0].cpu(), c.kc[:, 2]) and torch.equal(c.v[:, 0].cpu(), c.vc[:, 2])

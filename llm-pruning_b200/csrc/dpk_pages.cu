@@ -472,9 +472,10 @@ struct PoolParams {
 // flight before the stores.  The list's length is known on the device only, so a fixed grid walks it.
 constexpr int kMoveBytes = 16384;
 
+// The list is written while this kernel is already resident, so its pointers are not __restrict__: loads that
+// the compiler may take for those of a constant could be moved ahead of the wait.
 __global__ void __launch_bounds__(256)
-page_move_kernel(const PageMove* __restrict__ moves, const int32_t* __restrict__ count, const PoolParams pp,
-                 int page)
+page_move_kernel(const PageMove* moves, const int32_t* count, const PoolParams pp, int page)
 {
     asm volatile("griddepcontrol.wait;" ::: "memory");       // started while the bookkeeping still runs
     const int pieces = (page * pp.row_bytes + kMoveBytes - 1) / kMoveBytes;

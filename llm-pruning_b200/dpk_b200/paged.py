@@ -103,7 +103,7 @@ def _token_rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     ts = t.stride(0) if n > 1 else heads * D
     if not ((D == 1 or t.stride(2) == 1) and (heads == 1 or t.stride(1) == D) and ts >= heads * D
             and ts % 8 == 0 and t.data_ptr() % 16 == 0):
-        t = t.contiguous()
+        t = t.clone(memory_format=torch.contiguous_format)       # of a contiguous one too: it starts off 16 bytes
         ts = heads * D
     return t, ts
 

@@ -234,7 +234,7 @@ def _rope(dev, q, k, v, positions, inv_freq, sections, axis_map, interleaved, at
     if v is not None:
         vc, v_ts = _token_rows(v)
         if v_ts != kv_ts:
-            kc, vc = k.contiguous(), v.contiguous()
+            kc, vc = kc.contiguous(), vc.contiguous()
             kv_ts = Hk * D
     if q_out is None:
         q_out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((n, Hq, D))

@@ -304,3 +304,42 @@ def test_page_compact_reports_entries_of_pages_that_nobody_holds(ops):
     assert live.tolist() == [1] and c.refs.tolist() == [1] + [0] * 7
     assert c.table.tolist() == [[-1] * 3, [0, -1, -1], [-1] * 3, [-1] * 3]
     assert torch.equal(c.k[:, 0].cpu(), c.kc[:, 2]) and torch.equal(c.v[:, 0].cpu(), c.vc[:, 2])
+
+
+# ------------------------------------------------------------------ alignment (GPU)
+
+def shifted(t):
+    """The same values, contiguous, one element off an aligned address."""
+    room = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")
+    room[1:] = t.cuda().flatten()
+    return room[1:].view(t.shape)
+
+
+@pytest.mark.gpu
+def test_paged_operators_take_unaligned_queries_keys_and_values(ops):
+    b, near = rope_case(4)
+    d = cuda(b)
+    state = (d["k"], d["v"], d["table"], d["lens"], d["start"])
+    q = ops.rope_append_paged(shifted(b["q"]), shifted(b["kn"]), shifted(b["vn"]), d["pos"], d["inv"], *state,
+                              sections=b["sections"])
+    check_rotated(q, b["q"], b, near)
+    wrote = d["k"].clone(), d["v"].clone()
+    q2, k2 = ops.rope_axes(shifted(b["q"]), shifted(b["kn"]), d["pos"], d["inv"], b["sections"])
+    assert torch.equal(q2, q)
+    # k and v of different strides, one of them off its alignment
+    n = b["q"].shape[0]
+    wide = torch.zeros(n, 8 * 128 + 64, dtype=FP, device="cuda")
+    wide[:, :1024] = d["vn"].flatten(1)
+    for x in (d["k"], d["v"]):
+        x.zero_()
+    for s, t in (("k", b["k"]), ("v", b["v"])):
+        d[s].copy_(t)
+    ops.rope_append_paged(d["q"], shifted(b["kn"]), wide[:, :1024].view(n, 8, 128), d["pos"], d["inv"], *state,
+                          sections=b["sections"])
+    assert torch.equal(d["k"], wrote[0]) and torch.equal(d["v"], wrote[1])
+    at = b["lens"][0] - n
+    assert torch.equal(d["k"][b["table"][0, at // 8].long(), at % 8], k2[0])
+    a = make([3, 2], [30, 9], 16, 4, 2, 64, BF, seed=47)
+    e = cuda(a)
+    got, _ = ops.attention_paged(shifted(a["q"]), e["k"], e["v"], e["table"], e["lens"], e["start"])
+    check_attention(got, a)

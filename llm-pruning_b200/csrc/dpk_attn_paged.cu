@@ -656,7 +656,9 @@ int dpk_attn_paged(const void* Q, const void* K, const void* V, const int32_t* p
                    int64_t page_token_stride, int64_t table_stride, void* workspace, size_t workspace_bytes,
                    void* stream)
 {
-    DPK_REQUIRE(Q && K && V && O && page_table && kv_lens && query_start, "NULL tensor");
+    // a pool without pages and a table without entries have no address; nothing reads them
+    DPK_REQUIRE(Q && ((K && V) || P == 0) && O && (page_table || W == 0 || S == 0) && (kv_lens || S == 0) && query_start,
+                "NULL tensor");
     DPK_REQUIRE(dtype == DPK_F16 || dtype == DPK_BF16, "dtype must be DPK_F16 or DPK_BF16");
     DPK_REQUIRE(N >= 0 && N < (1ll << 31) && S >= 0 && W >= 0 && P >= 0 && Hq > 0 && Hk > 0, "bad shape");
     DPK_REQUIRE(D == 64 || D == 128, "head_dim %d not supported (64 or 128)", D);
@@ -689,8 +691,8 @@ int dpk_attn_paged(const void* Q, const void* K, const void* V, const int32_t* p
     DPK_REQUIRE(aligned16(workspace), "workspace must be 16-byte aligned");
     PagedParams p;
     p.Q = static_cast<const uint8_t*>(Q);
-    p.K = static_cast<const uint8_t*>(K);
-    p.V = static_cast<const uint8_t*>(V);
+    p.K = static_cast<const uint8_t*>(P > 0 ? K : Q);          // tensor maps are made all the same
+    p.V = static_cast<const uint8_t*>(P > 0 ? V : Q);
     p.O = static_cast<uint8_t*>(O);
     p.table = page_table;
     p.kv_lens = kv_lens;

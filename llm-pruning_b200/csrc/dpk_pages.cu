@@ -538,9 +538,9 @@ static int move_pages(const PageState& st, const PoolParams& pp, int64_t most, i
 }
 
 static int pool_params(PoolParams& pp, void* k, void* v, int layers, int64_t layer_stride, int64_t page_stride,
-                       int page, int row_elems)
+                       int P, int page, int row_elems)
 {
-    DPK_REQUIRE(k && v, "NULL tensor");
+    DPK_REQUIRE((k && v) || P == 0, "NULL tensor");          // a pool of nothing has no address
     DPK_REQUIRE(layers > 0 && row_elems > 0 && row_elems % 8 == 0, "a token's row must be a multiple of 8 elements");
     DPK_REQUIRE(page_stride % 8 == 0 && layer_stride % 8 == 0 && aligned16(k) && aligned16(v),
                 "pools must be 16-byte aligned with strides of multiples of 8 elements");
@@ -558,8 +558,8 @@ static int pool_params(PoolParams& pp, void* k, void* v, int layers, int64_t lay
 static int page_state(PageState& st, int32_t* table, int64_t table_stride, int32_t* lens, int32_t* refs, int S,
                       int W, int P, int page)
 {
-    DPK_REQUIRE(table && lens && refs, "NULL tensor");
     DPK_REQUIRE(S >= 0 && W >= 0 && P >= 0 && page > 0, "bad shape");
+    DPK_REQUIRE((table || S == 0 || W == 0) && (lens || S == 0) && (refs || P == 0), "NULL tensor");
     DPK_REQUIRE(table_stride >= W, "table_stride is smaller than a row");
     DPK_REQUIRE(static_cast<int64_t>(W) * page < (1ll << 31), "a row of the table holds 2^31 tokens or more");
     DPK_REQUIRE(P <= (1 << 30) && S <= (1 << 24) && static_cast<int64_t>(S) * (W + 1) < (1ll << 31),
@@ -615,10 +615,10 @@ int dpk_page_extend(int32_t* table, int64_t table_stride, int32_t* lens, int32_t
     PoolParams pp;
     int rc = page_state(st, table, table_stride, lens, refs, S, W, P, page);
     if (rc) return rc;
-    rc = pool_params(pp, k, v, layers, layer_stride, page_stride, page, row_elems);
+    rc = pool_params(pp, k, v, layers, layer_stride, page_stride, P, page, row_elems);
     if (rc) return rc;
-    DPK_REQUIRE(add && granted, "NULL tensor");
     if (S == 0) return DPK_OK;
+    DPK_REQUIRE(add && granted, "NULL tensor");
     const size_t need = dpk_page_workspace_bytes(S, 0, 0);
     DPK_REQUIRE(workspace && workspace_bytes >= need, "workspace of %zu bytes needed, %zu given", need, workspace_bytes);
     rc = page_status(st);
@@ -679,7 +679,7 @@ int dpk_page_copy(void* k, void* v, int layers, int64_t layer_stride, int64_t pa
     DPK_REQUIRE(P >= 0 && page > 0, "bad shape");
     int rc = page_state(st, &none, 0, &none, &none, 0, 0, P, page);
     if (rc) return rc;
-    rc = pool_params(pp, k, v, layers, layer_stride, page_stride, page, row_elems);
+    rc = pool_params(pp, k, v, layers, layer_stride, page_stride, P, page, row_elems);
     if (rc) return rc;
     DPK_REQUIRE(n >= 0, "bad shape");
     if (n == 0) return DPK_OK;
@@ -704,7 +704,7 @@ int dpk_page_compact(void* k, void* v, int layers, int64_t layer_stride, int64_t
     PoolParams pp;
     int rc = page_state(st, table, table_stride, lens, refs, S, W, P, page);
     if (rc) return rc;
-    rc = pool_params(pp, k, v, layers, layer_stride, page_stride, page, row_elems);
+    rc = pool_params(pp, k, v, layers, layer_stride, page_stride, P, page, row_elems);
     if (rc) return rc;
     DPK_REQUIRE(live, "NULL tensor");
     const size_t need = dpk_page_workspace_bytes(0, P, 0);

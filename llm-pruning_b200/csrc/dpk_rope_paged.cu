@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 5) rope_paged_kernel(const Ro
         const int t = static_cast<int>(job / split), part = static_cast<int>(job - static_cast<int64_t>(t) * split);
         // where the token's k and v go: element offset in the pools, -1 nowhere
         int64_t row = -1;
-        if (p.k_pages) {
+        if (p.v) {
             if (t >= p.qstart[p.S]) continue;            // behind the last sequence: left as it is
             int lo = 0, hi = p.S;                        // last sequence that starts at or before t
             while (hi - lo > 1) {
@@ -188,7 +188,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 5) rope_paged_kernel(const Ro
                     uint8_t* dst;
                     if (head < p.Hq) {
                         dst = p.q_out + (t * p.qo_ts + static_cast<int64_t>(head) * p.D) * 2;
-                    } else if (!p.k_pages) {
+                    } else if (!p.v) {
                         dst = p.k_out + (static_cast<int64_t>(t) * p.Hk + head - p.Hq) * p.D * 2;
                     } else if (row < 0) {
                         continue;
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 5) rope_paged_kernel(const Ro
         }
     }
     // starts that no token looked at: sequences without a row, a first start that is not 0
-    if (p.k_pages) {
+    if (p.v) {
         const int64_t all = static_cast<int64_t>(gridDim.x) * (kRopeWarps * 32);
         for (int64_t s = static_cast<int64_t>(blockIdx.x) * (kRopeWarps * 32) + threadIdx.x; s < p.S; s += all) {
             const int begin = p.qstart[s], end = p.qstart[s + 1];
@@ -262,6 +262,8 @@ int dpk_rope_append_paged_granted(const void* q, const void* k, const void* v, v
 {
     DPK_REQUIRE(q && k && q_out && positions && inv_freq, "NULL tensor");
     DPK_REQUIRE((k_pages == nullptr) == (v_pages == nullptr), "k_pages and v_pages go together");
+    // a cache of no pages has no address, but a state: its tokens have no place, which is reported
+    const bool cached = k_pages || (query_start && P == 0 && !k_out);
     DPK_REQUIRE(dtype == DPK_F16 || dtype == DPK_BF16, "dtype must be DPK_F16 or DPK_BF16");
     DPK_REQUIRE(N >= 0 && Hq > 0 && Hk > 0, "bad shape");
     DPK_REQUIRE(D > 0 && D % 16 == 0 && D <= 1024, "head_dim=%d must be a multiple of 16 up to 1024", D);
@@ -275,8 +277,8 @@ int dpk_rope_append_paged_granted(const void* q, const void* k, const void* v, v
                 "token strides must cover a token's heads and be multiples of 8 elements");
     DPK_REQUIRE(axes == 1 || axis_stride >= N, "positions of an axis overlap the next axis");
     RopePagedParams p;
-    if (k_pages) {
-        DPK_REQUIRE(v && table && kv_lens && query_start, "NULL tensor");
+    if (cached) {
+        DPK_REQUIRE(v && (table || W == 0 || S == 0) && (kv_lens || S == 0) && query_start, "NULL tensor");
         DPK_REQUIRE(S >= 0 && W >= 0 && P >= 0 && page_size > 0 && table_stride >= W, "bad shape");
         DPK_REQUIRE(int64_t(W) * page_size < (1ll << 31), "a row of the table holds 2^31 tokens or more");
         DPK_REQUIRE(page_token_stride >= int64_t(Hk) * D && page_token_stride % 8 == 0 && page_stride % 8 == 0,
@@ -300,7 +302,7 @@ int dpk_rope_append_paged_granted(const void* q, const void* k, const void* v, v
     if (N == 0) return DPK_OK;
     p.q = static_cast<const uint8_t*>(q);
     p.k = static_cast<const uint8_t*>(k);
-    p.v = k_pages ? static_cast<const uint8_t*>(v) : nullptr;
+    p.v = cached ? static_cast<const uint8_t*>(v) : nullptr;
     p.q_out = static_cast<uint8_t*>(q_out);
     p.k_out = static_cast<uint8_t*>(k_out);
     p.k_pages = static_cast<uint8_t*>(k_pages);

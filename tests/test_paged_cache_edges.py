@@ -343,3 +343,50 @@ def test_paged_operators_take_unaligned_queries_keys_and_values(ops):
     e = cuda(a)
     got, _ = ops.attention_paged(shifted(a["q"]), e["k"], e["v"], e["table"], e["lens"], e["start"])
     check_attention(got, a)
+
+
+# ------------------------------------------------------------------ empty states (GPU)
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S,W,P", [(0, 4, 6), (3, 0, 6), (3, 4, 0), (0, 0, 0), (0, 4, 0), (3, 0, 0)])
+def test_paged_operators_of_empty_states(ops, S, W, P):
+    k = torch.zeros(2, P, 8, 2, 64, dtype=BF, device="cuda")
+    v = torch.zeros_like(k)
+    table = torch.full((S, W), -1, dtype=torch.int32, device="cuda")
+    lens, refs = torch.zeros(S, dtype=torch.int32, device="cuda"), torch.zeros(P, dtype=torch.int32, device="cuda")
+    none = i32([])
+    granted = ops.page_extend(k, v, table, lens, refs, torch.zeros_like(lens))
+    assert granted.dtype is torch.bool and granted.tolist() == [True] * S
+    granted = ops.page_extend(k, v, table, lens, refs, torch.ones_like(lens))
+    assert granted.tolist() == [False] * S and lens.tolist() == [0] * S
+    assert ops.page_compact(k, v, table, lens, refs).tolist() == [0]
+    ops.page_trim(table, lens, refs, torch.arange(S, dtype=torch.int32, device="cuda"), page_size=8)
+    ops.page_trim(table, lens, refs, none, page_size=8)
+    assert ops.page_fork(table, lens, refs, none, none, 8).shape == (0,)
+    ops.page_copy(k, v, none, none)
+    assert ops.device_status() == 0
+    if P == 0:
+        ops.page_copy(k, v, i32([0]), i32([1]))
+        assert ops.device_status() == 16105
+    if S == 0:
+        ops.page_trim(table, lens, refs, i32([0]), page_size=8)
+        assert ops.device_status() == 16105
+        assert ops.page_fork(table, lens, refs, i32([0]), i32([1]), 8).tolist() == [False]
+        assert ops.device_status() == 16105
+    # no token is cached: every row sees nothing
+    n = max(S, 1)
+    start = i32(list(range(S + 1)))
+    q = torch.ones(n, 4, 64, dtype=BF, device="cuda")
+    for most in (1, 64):
+        poison(q, 7.0)
+        out, _ = ops.attention_paged(q, k[0], v[0], table, lens, start, max_query_len=most)
+        assert (out == 0).all() and ops.device_status() == 0
+    # a token without a place in the pages is reported, its query turned all the same
+    pos, inv = torch.zeros(1, n, dtype=torch.int64, device="cuda"), torch.ones(32, device="cuda")
+    out = ops.rope_append_paged(q, q[:, :2], q[:, :2], pos, inv, k[0], v[0], table, lens, start)
+    if S:
+        assert torch.equal(out, q) and ops.device_status() == 15105
+        lens.fill_(5)                                  # lengths that the state cannot hold
+        for most in (1, 64):
+            out, _ = ops.attention_paged(q, k[0], v[0], table, lens, start, max_query_len=most)
+            assert (out == 0).all() and ops.device_status() % 1000 == 105

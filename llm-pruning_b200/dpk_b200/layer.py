@@ -161,7 +161,7 @@ class RoutedDecoderLayer:
         ``positions [axes,N]`` or ``[N]`` and ``inv_freq`` as :func:`ops.rope_append_paged` takes them, with
         its ``sections`` / ``axis_map`` / ``interleaved`` / ``attention_scale`` / ``granted``; ``layer``: this
         layer's number in the cache.  Tokens of a row that the cache refused may be sent: they change
-        nothing in it."""
+        nothing in it.  Rows behind ``query_start``'s end are padding: they see no key."""
         f = self.front
         N = x.shape[0]
         x3 = x[None]
@@ -171,21 +171,24 @@ class RoutedDecoderLayer:
         if f["ar"] is not None:
             am = am[..., f["ar"][0]:f["ar"][1]]
         self._mark("route1")
-        q, k, v = self.project_qkv(h, am)
+        # Buffers of this call alone, for q, k and v and for the attention's output: steps differ in size, and
+        # one that was captured would go on writing to a buffer of the layer's after a larger step replaced it.
+        q, k, v = self.project_qkv(h, am, x.new_empty(N * (self.Hq + 2 * self.Hk) * self.D))
         # rows of routed-out head groups were not projected: they are turned as they are and never attended
         q = cache.rope_update(layer, q[0], k[0], v[0], positions, inv_freq, query_start, q_out=q[0], **rope)
         self._mark("qkv")
-        attn = cache.attend(layer, q, query_start, am[0], max_query_len=max_query_len,
-                            out=self._attention_out(1, N, q)[0])
+        # zero where it is not computed: a padded step's rows behind the last sequence depend on x alone
+        attn = cache.attend(layer, q, query_start, am[0], max_query_len=max_query_len)
         self._mark("attn")
         out, fm, fm_all = self._after_attention(x3, attn[None], am, {})
         if return_masks == "full":
             return out[0], am_all[0], fm_all[0]
         return (out[0], am[0], fm[0]) if return_masks else out[0]
 
-    def project_qkv(self, h: torch.Tensor, attn_mask: torch.Tensor):
+    def project_qkv(self, h: torch.Tensor, attn_mask: torch.Tensor, into: Optional[torch.Tensor] = None):
         """``q [B,T,Hq,D]``, ``k, v [B,T,Hk,D]`` of ``h [B,T,H]``; rows of q whose head group is
-        routed out are left unwritten (attention never reads them)."""
+        routed out are left unwritten (attention never reads them).  ``into``: memory for the stacked
+        result instead of the layer's own buffer."""
         B, T, _ = h.shape
         qd, kd = self.Hq * self.D, self.Hk * self.D
         if not self.fold_qkv:
@@ -199,9 +202,11 @@ class RoutedDecoderLayer:
         stacked = torch.cat([m.repeat_interleave(per_head_group, dim=-1),
                              torch.ones((B, T, 2 * kd // G), dtype=torch.bool, device=h.device)], dim=-1)
         width = qd + 2 * kd
-        if self._qkv_out is None or self._qkv_out.numel() < B * T * width or self._qkv_out.dtype != h.dtype:
-            self._qkv_out = torch.empty(B * T * width, dtype=h.dtype, device=h.device)
-        out = self._qkv_out[:B * T * width].view(B * T, width)
+        if into is None:
+            if self._qkv_out is None or self._qkv_out.numel() < B * T * width or self._qkv_out.dtype != h.dtype:
+                self._qkv_out = torch.empty(B * T * width, dtype=h.dtype, device=h.device)
+            into = self._qkv_out
+        out = into[:B * T * width].view(B * T, width)
         ops.gemm_mn(h, self.wqkv, stacked, D=out)
         out = out.view(B, T, width)
         return (out[..., :qd].view(B, T, self.Hq, self.D),

@@ -390,3 +390,81 @@ def test_paged_operators_of_empty_states(ops, S, W, P):
         for most in (1, 64):
             out, _ = ops.attention_paged(q, k[0], v[0], table, lens, start, max_query_len=most)
             assert (out == 0).all() and ops.device_status() % 1000 == 105
+
+
+# ------------------------------------------------------------------ a layer's captured steps (GPU)
+
+def small_layer(seed=61, max_tokens=300):
+    from dpk_b200.layer import RoutedDecoderLayer
+
+    g = torch.Generator().manual_seed(seed)
+    H, Hq, Hk, D, I, NGF, R = 256, 8, 2, 64, 1024, 8, 16
+    rand = lambda *shape, std=0.05: (torch.randn(*shape, generator=g) * std).to(BF).cuda()
+    layer = RoutedDecoderLayer(rand(Hq * D, H), rand(Hk * D, H), rand(Hk * D, H), rand(H, Hq * D), rand(I, H),
+                               rand(I, H), rand(H, I), num_q_heads=Hq, num_kv_heads=Hk, head_dim=D, attn_groups=Hk,
+                               ffn_groups=NGF, max_tokens=max_tokens)
+    router = lambda ng: (rand(R, H), rand(R, std=0.1), rand(2 * ng, R, std=0.25), rand(2 * ng, std=0.1))
+    layer.set_front_end(router(Hk), router(NGF), torch.ones(H, dtype=BF, device="cuda"),
+                        torch.ones(H, dtype=BF, device="cuda"), 1e-5)
+    return layer, g
+
+
+def new_cache(rows=3):
+    from dpk_b200.wide import PagedKVCache
+    return PagedKVCache(1, 80, 16, 2, 64, rows, 320, BF, "cuda")
+
+
+@pytest.mark.gpu
+def test_forward_cached_captured_step_owns_its_buffers(ops):
+    """A step captured for a few tokens, then a larger one that is not captured, then the captured one again:
+    what the larger step left behind and what others allocated meanwhile stays as it is."""
+    layer, g = small_layer()
+    cache, twin = new_cache(), new_cache()
+    inv = (10000.0 ** (-torch.arange(32, dtype=torch.float64) / 32)).float().cuda()
+    x1 = torch.randn(3, 256, generator=g).to(BF).cuda()
+    x2 = torch.randn(280, 256, generator=g).to(BF).cuda()
+    one, start1 = i32([1, 1, 1]), i32([0, 1, 2, 3])
+    many, start2 = i32([200, 0, 80]), i32([0, 200, 200, 280])
+    pos2 = torch.cat([torch.arange(200), torch.arange(80)]).cuda() + 1
+
+    def step(c, x, add, start, pos, most):
+        c.extend(add)
+        return layer.forward_cached(x, c.lengths - 1 if pos is None else pos, inv, c, 0, start, max_query_len=most)
+    step(twin, x1, one, start1, None, 1)              # loads what is loaded at first use
+    twin.free(i32([0, 1, 2]))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(cache, x1, one, start1, None, 1)
+    graph.replay()
+    a1 = out.clone()
+    a2 = step(cache, x2, many, start2, pos2, 200)
+    others = [torch.full((n,), 5.0, dtype=BF, device="cuda") for n in (3 * 768, 3 * 512, 4096, 280 * 768, 280 * 512)
+              for _ in range(6)]
+    graph.replay()
+    a3 = out.clone()
+    torch.cuda.synchronize()
+    assert all((t == 5).all() for t in others)
+    b1 = step(twin, x1, one, start1, None, 1)
+    b2 = step(twin, x2, many, start2, pos2, 200)
+    b3 = step(twin, x1, one, start1, None, 1)
+    assert torch.equal(a1, b1) and torch.equal(a2, b2) and torch.equal(a3, b3)
+
+
+@pytest.mark.gpu
+def test_forward_cached_rows_behind_the_last_sequence(ops):
+    """A padded step: the rows behind the last sequence get no attention, whatever memory held before."""
+    layer, g = small_layer()
+    inv = torch.ones(32, device="cuda")
+    x = torch.randn(9, 256, generator=g).to(BF).cuda()
+    pos = torch.zeros(9, dtype=torch.int64, device="cuda")
+    outs = []
+    for value in (math.nan, 3.0):
+        cache = new_cache()
+        cache.extend(i32([2, 0, 3]))
+        for width in (9 * 512, 9 * 768):
+            poison(torch.empty(width, dtype=BF, device="cuda"), value)
+        if getattr(layer, "_attn_out", None) is not None:
+            layer._attn_out.fill_(value)
+        outs.append(layer.forward_cached(x, pos, inv, cache, 0, i32([0, 2, 2, 5]), max_query_len=3))
+    assert torch.isfinite(outs[0]).all() and torch.equal(outs[0], outs[1])

@@ -167,6 +167,7 @@ def attention_paged(Q: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tenso
     most = n if max_query_len is None else int(max_query_len)
     if n and most < 1:
         raise ValueError("max_query_len must be at least 1")
+    most = min(most, 2 ** 31 - 1)        # what the C argument holds
     if n == 0 or S == 0:                 # nothing to attend: every row is behind the last sequence
         if clear:
             O.zero_()

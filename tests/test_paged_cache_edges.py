@@ -468,3 +468,15 @@ def test_forward_cached_rows_behind_the_last_sequence(ops):
             layer._attn_out.fill_(value)
         outs.append(layer.forward_cached(x, pos, inv, cache, 0, i32([0, 2, 2, 5]), max_query_len=3))
     assert torch.isfinite(outs[0]).all() and torch.equal(outs[0], outs[1])
+
+
+# ------------------------------------------------------------------ bounds of arguments
+
+@pytest.mark.gpu
+def test_attention_paged_any_upper_bound_of_new_tokens(ops):
+    b = make([3, 40], [30, 9], 16, 4, 2, 64, BF, seed=48)
+    d = cuda(b)
+    want, _ = ops.attention_paged(d["q"], d["k"], d["v"], d["table"], d["lens"], d["start"], max_query_len=43)
+    for most in (2 ** 31 - 1, 2 ** 31, 2 ** 32 + 1, 2 ** 40):
+        got, _ = ops.attention_paged(d["q"], d["k"], d["v"], d["table"], d["lens"], d["start"], max_query_len=most)
+        assert torch.equal(got, want)

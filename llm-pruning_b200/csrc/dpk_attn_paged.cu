@@ -682,7 +682,8 @@ int dpk_attn_paged(const void* Q, const void* K, const void* V, const int32_t* p
     const PagedShape g = paged_shape(N, S, Hq, Hk, D, max_query_len, mask != nullptr, sm_total());
     const int workers = g.workers / sm_total() * sm_count();      // SMs left free by dpk_set_sm_margin
     const int64_t most = g.max_tiles * ((int64_t(W) * page_size + g.unit_keys - 1) / g.unit_keys + g.tile_gap);
-    DPK_REQUIRE(most < (1ll << 31), "too much work for one call: %lld tiles of up to %lld keys",
+    // places are 32-bit, and a worker's range may end a range behind the line (plan_range: below 2^16, or an equal share)
+    DPK_REQUIRE(most < (1ll << 31) - (1 << 16), "too much work for one call: %lld tiles of up to %lld keys",
                 (long long)g.max_tiles, (long long)W * page_size);
     DPK_REQUIRE((g.max_tiles + 1) * g.workers < (1ll << 31), "too many tiles for one call");
     DPK_REQUIRE(int64_t(Hq) * N < (1ll << 31), "too many rows for one call");

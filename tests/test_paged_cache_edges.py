@@ -480,3 +480,21 @@ def test_attention_paged_any_upper_bound_of_new_tokens(ops):
     for most in (2 ** 31 - 1, 2 ** 31, 2 ** 32 + 1, 2 ** 40):
         got, _ = ops.attention_paged(d["q"], d["k"], d["v"], d["table"], d["lens"], d["start"], max_query_len=most)
         assert torch.equal(got, want)
+
+
+def test_attention_paged_refuses_work_near_the_end_of_32_bits(ops):
+    """A worker's range ends at most a few ten thousand places behind the line's end, which has to fit too."""
+    import ctypes
+
+    from dpk_b200 import _native as N
+    lib = N.load()
+    buf = (ctypes.c_uint8 * 512)()
+    p = (ctypes.addressof(buf) + 255) & ~255
+    # 8 heads, S sequences of one token: 8 * (S + S // 16) tiles of W * 8 / 32 + 1 places
+    S, W = 496, 4 * 509355                              # 4216 tiles of 509355 + 1 places: 2^31 - 39 thousand
+    tiles = 8 * (S // 16 + S)
+    places = tiles * ((W * 8 + 31) // 32 + 1)
+    assert 2 ** 31 - 2 ** 16 <= places < 2 ** 31
+    rc = lib.dpk_attn_paged(p, p, p, p, p, p, None, p, S, S, W, 8, 8, 8, 8, 64, 1, 0.1, 1, N.BF16, 1, 0, 0, 0, 0, 0, p, 0,
+                            None)
+    assert rc == N.ERR_INVALID and "too much work" in N.last_error()

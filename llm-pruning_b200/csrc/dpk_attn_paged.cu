@@ -7,9 +7,12 @@
 // K and V are read through the page table; rows whose head group is routed out, and rows that see
 // no key, are zero.
 //
-// Three launches: paged_plan_kernel cuts the work (dpk_attn_paged.cuh), an attention kernel runs
-// it, paged_join_kernel joins the tiles that several workers shared and writes the zero rows.  Each
-// is started while its predecessor still runs.
+// Two to four launches: paged_rows_kernel lists the active rows (chunks with a mask), paged_plan_kernel
+// cuts the work (dpk_attn_paged.cuh; lists of up to kPwTiles or kPtTiles tiles are made inside the
+// attention kernel instead), an attention kernel runs it, paged_join_kernel joins the tiles that several
+// workers shared and writes the zero rows.  Each is started while its predecessor still runs.
+//
+// Scores that are NaN or +inf, and rows that see -inf alone, give NaN, however the work was cut.
 //
 // The attention kernel here gives every WARP a range of 32-key units.  Its tile is 16 rows, so the
 // Hq/Hk heads of up to 16 / (Hq/Hk) new tokens read every K/V byte once; K and V arrive through a
@@ -136,11 +139,12 @@ __device__ __forceinline__ uint32_t pw_off(int r, int c)
     return static_cast<uint32_t>(r * (D * 2) + ((c ^ (r & 7)) << 4));
 }
 
-// Up to kPwTiles tiles (a decode step of 16 sequences with 8 KV heads) the attention kernel makes the work
-// list itself, every CTA for its own use in shared memory behind the rings: that saves a launch of a
-// kernel that takes as long as a small step's attention (8 tiles: 11.4 us on the device instead of 12.5,
-// 22.7 a call instead of 26.2).  A CTA of 128 threads takes longer over a long list than the launch does
-// (128 tiles: the same on the device; 512: 262 us instead of 258).
+// Up to kPwTiles tiles by the host's bound, Hk * (N * rep / 16 + S) (a decode step of 15 sequences with 32
+// query and 8 KV heads, of 16 with 16 and 8), the attention kernel makes the work list itself, every CTA for
+// its own use in shared memory behind the rings: that saves a launch of a kernel that takes as long as a
+// small step's attention (8 tiles: 11.4 us on the device instead of 12.5, 22.7 a call instead of 26.2).  A
+// CTA of 128 threads takes longer over a long list than the launch does (128 tiles: the same on the
+// device; 512: 262 us instead of 258).
 constexpr int kPwTiles = 144;
 
 template <int D, bool kBf16, bool kPlanHere>

@@ -60,7 +60,7 @@ struct PagedParams {
     int32_t* start;         // [tiles + 1] place of each tile's first unit
     PagedTile* tile;        // [tiles]
     PagedTile* slot;        // [max_tiles] with `rows`: tiles as paged_rows_kernel leaves them
-    int32_t* first_tile;    // [S * Hk + 1] running number of tiles before dropping empty ones
+    int32_t* first_tile;    // [S * Hk] running number of tiles before dropping empty ones; more than kPlanItems only
     int32_t* rows;          // [Hk][N * rep] active rows of each (sequence, KV head), or NULL: all rows
     int32_t* row_count;     // [S * Hk] with `rows`
     PagedBorder* border;    // [workers]

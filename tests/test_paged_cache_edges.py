@@ -409,6 +409,18 @@ def small_layer(seed=61, max_tokens=300):
     return layer, g
 
 
+def alike(layer, a, b):
+    """Two outputs of ``layer`` on the same input.  Its down projection adds up to 8 parts of a sum to one 32-bit
+    accumulator in any order, and the residual: 9 additions, each off by 2^-24 of what is summed at most, before
+    one rounding to 16 bits.  (The output projection's two parts give the same bits in either order.)  What is summed
+    is below sum_i |wd_i| |g_i| |u_i| with |silu(g) u| <= |g| |u|, |g| <= |wg_i| |h|, |u| <= |wu_i| |h|, and |h| = sqrt(256)
+    of the normed input within its own rounding."""
+    f = layer.ffn
+    most = f.wd.float().abs() @ (f.wg.float().norm(dim=1) * f.wu.float().norm(dim=1)) * 256 * (1 + 2.0 ** -6)
+    size = torch.maximum(a.float().abs(), b.float().abs())
+    return bool(((a.float() - b.float()).abs() <= 2 * 9 * 2.0 ** -24 * (2 * most + size) + 2 * u_of(BF) * size).all())
+
+
 def new_cache(rows=3):
     from dpk_b200.wide import PagedKVCache
     return PagedKVCache(1, 80, 16, 2, 64, rows, 320, BF, "cuda")
@@ -448,7 +460,7 @@ def test_forward_cached_captured_step_owns_its_buffers(ops):
     b1 = step(twin, x1, one, start1, None, 1)
     b2 = step(twin, x2, many, start2, pos2, 200)
     b3 = step(twin, x1, one, start1, None, 1)
-    assert torch.equal(a1, b1) and torch.equal(a2, b2) and torch.equal(a3, b3)
+    assert alike(layer, a1, b1) and alike(layer, a2, b2) and alike(layer, a3, b3)
 
 
 @pytest.mark.gpu
@@ -467,7 +479,7 @@ def test_forward_cached_rows_behind_the_last_sequence(ops):
         if getattr(layer, "_attn_out", None) is not None:
             layer._attn_out.fill_(value)
         outs.append(layer.forward_cached(x, pos, inv, cache, 0, i32([0, 2, 2, 5]), max_query_len=3))
-    assert torch.isfinite(outs[0]).all() and torch.equal(outs[0], outs[1])
+    assert torch.isfinite(outs[0]).all() and alike(layer, outs[0], outs[1])
 
 
 # ------------------------------------------------------------------ bounds of arguments
@@ -498,3 +510,71 @@ def test_attention_paged_refuses_work_near_the_end_of_32_bits(ops):
     rc = lib.dpk_attn_paged(p, p, p, p, p, p, None, p, S, S, W, 8, 8, 8, 8, 64, 1, 0.1, 1, N.BF16, 1, 0, 0, 0, 0, 0, p, 0,
                             None)
     assert rc == N.ERR_INVALID and "too much work" in N.last_error()
+
+
+# ------------------------------------------------------------------ rarer dispatch paths (GPU)
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("masked", [False, True])
+def test_attention_paged_more_pairs_than_shared_memory_holds(ops, masked):
+    """600 sequences of 8 KV heads: the tiles' numbers are in the workspace."""
+    new = [1 + i % 2 for i in range(600)]
+    b = make(new, [i * 5 % 23 for i in range(600)], 8, 8, 8, 64, BF, seed=49)
+    mask = torch.rand(b["q"].shape[0], 4, generator=b["gen"]) < 0.6 if masked else None
+    d = cuda(b)
+    for most in (2, 40):
+        got, _ = ops.attention_paged(d["q"], d["k"], d["v"], d["table"], d["lens"], d["start"],
+                                     None if mask is None else mask.cuda(), max_query_len=most)
+        check_attention(got, b, mask)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("rep,D,dtype", [(17, 64, BF), (32, 128, FP), (128, 64, BF)])
+def test_attention_paged_many_query_heads_per_kv_head(ops, rep, D, dtype, masked):
+    """More rows a token than the warp kernel's tile has: single tokens go to the chunk kernel."""
+    for new, cached in (([1, 1, 1], [70, 0, 333]), ([5, 1, 20], [9, 64, 200])):
+        b = make(new, cached, 16, 2 * rep, 2, D, dtype, seed=50 + rep)
+        mask = torch.rand(sum(new), 2 * rep, generator=b["gen"]) < 0.5 if masked else None
+        d = cuda(b)
+        for most in (1, max(new)):
+            got, _ = ops.attention_paged(d["q"], d["k"], d["v"], d["table"], d["lens"], d["start"],
+                                         None if mask is None else mask.cuda(), max_query_len=most)
+            check_attention(got, b, mask)
+
+
+# ------------------------------------------------------------------ pools beyond 2^31 elements (GPU)
+
+@pytest.mark.gpu
+def test_rope_and_pages_offsets_beyond_32_bits(ops):
+    """Writes, copies and moves between pages 4.4 GB apart in one pool of two-byte elements."""
+    page, Hk, D = 16, 2, 128
+    P = 2 ** 31 // (page * Hk * D) + 8
+    k = torch.zeros(P, page, Hk, D, dtype=BF, device="cuda")
+    v = torch.zeros(P, page, Hk, D, dtype=BF, device="cuda")
+    g = torch.Generator().manual_seed(62)
+    q, kn, vn = (torch.randn(3, h, D, generator=g).to(BF).cuda() for h in (4, Hk, Hk))
+    # three tokens: in the last page, in the first one, across the border of two far pages
+    table, lens, start = i32([[P - 1, -1], [0, -1], [1, P - 3]]), i32([4, 9, 17]), i32([0, 1, 2, 3])
+    pos = torch.arange(3, device="cuda")[None]
+    inv = torch.ones(D // 2, device="cuda")
+    ops.rope_append_paged(q, kn, vn, pos, inv, k, v, table, lens, start)
+    kr = ops.rope_axes(q, kn, pos, inv)[1]
+    places = [(P - 1, 3), (0, 8), (P - 3, 0)]
+    for t, at in enumerate(places):
+        assert torch.equal(k[at], kr[t]) and torch.equal(v[at], vn[t])
+        k[at], v[at] = 0, 0
+    assert not k.any() and not v.any()
+    for at in places:
+        k[at], v[at] = 1, 2
+    ops.page_copy(k, v, i32([P - 1, 0]), i32([3, P - 2]))
+    assert torch.equal(k[3], k[P - 1]) and torch.equal(v[P - 2], v[0]) and torch.equal(k[P - 2], k[0])
+    for p in (3, P - 2):
+        k[p], v[p] = 0, 0
+    refs = torch.zeros(P, dtype=torch.int32, device="cuda")
+    refs[[P - 1, 0, 1, P - 3]] = 1
+    lens = i32([4, 9, 17])
+    live = ops.page_compact(k, v, table, lens, refs)
+    assert live.tolist() == [4] and table.tolist() == [[3, -1], [0, -1], [1, 2]]
+    for at in ((3, 3), (0, 8), (2, 0)):
+        assert (k[at] == 1).all() and (v[at] == 2).all()

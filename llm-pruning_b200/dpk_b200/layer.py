@@ -164,6 +164,11 @@ class RoutedDecoderLayer:
         nothing in it.  Rows behind ``query_start``'s end are padding: they see no key."""
         f = self.front
         N = x.shape[0]
+        if N == 0:                # every row refused, or nothing to do: there is nothing to launch
+            masks = [x.new_empty((0, f[router][2].shape[0] // 2), dtype=torch.bool) for router in ("attn", "ffn")]
+            if return_masks != "full":
+                masks = [m if r is None else m[:, r[0]:r[1]] for m, r in zip(masks, (f["ar"], f["fr"]))]
+            return (torch.empty_like(x), *masks) if return_masks else torch.empty_like(x)
         x3 = x[None]
         self._mark("start")
         am, h, _ = ops.router_norm(x3, *f["attn"], norm_weight=f["n1"], eps=f["eps"])

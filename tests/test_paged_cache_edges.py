@@ -482,6 +482,20 @@ def test_forward_cached_rows_behind_the_last_sequence(ops):
     assert torch.isfinite(outs[0]).all() and alike(layer, outs[0], outs[1])
 
 
+@pytest.mark.gpu
+def test_forward_cached_without_a_token(ops):
+    layer, _ = small_layer()
+    cache = new_cache()
+    assert cache.extend(i32([0, 0, 0])).all()
+    x, pos = torch.zeros(0, 256, dtype=BF, device="cuda"), torch.zeros(0, dtype=torch.int64, device="cuda")
+    args = (x, pos, torch.ones(32, device="cuda"), cache, 0, i32([0, 0, 0, 0]))
+    assert layer.forward_cached(*args).shape == (0, 256)
+    for which in (True, "full"):
+        out, am, fm = layer.forward_cached(*args, return_masks=which)
+        assert out.shape == (0, 256) and am.shape == (0, 2) and fm.shape == (0, 8)
+    assert (cache.ref_counts == 0).all()
+
+
 # ------------------------------------------------------------------ bounds of arguments
 
 @pytest.mark.gpu

@@ -382,7 +382,8 @@ int dpk_rope_append(void* q, void* k, const void* v, const void* cos, const void
  * Rows of O of routed-out heads and of tokens that see no key are zero; rows of no sequence (behind
  * query_start[S]) are left as they are, or zeroed with clear_tail.  What the cache holds behind
  * kv_lens, in pages no sequence holds, or in keys that a token may not see, has no influence (values
- * that a token may not see but another new token of its sequence may: finite values only).
+ * that a token may not see but another new token of its sequence may: finite values only).  Rows
+ * that see a score of NaN or +inf, or scores of -inf alone, are NaN.
  * max_query_len: an upper bound of n_s.  It chooses the kernel and the size of the workspace; a
  * sequence with more new tokens than it says is still computed.
  * Requirements: D in {64,128}, Hq % Hk == 0, Hq/Hk <= 128, Hq % NG == 0, page_size % 8 == 0, scale > 0.

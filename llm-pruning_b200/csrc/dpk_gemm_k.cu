@@ -8,8 +8,10 @@
 // group it loads the window's A columns with one TMA tile load, overwrites the rows
 // of tokens that do not use the group with zeros in shared memory, and issues the
 // UMMAs.  Groups that no token of the window uses are skipped entirely (loads and
-// MMAs).  There are no global atomics and the result is deterministic; the price is
-// that an inactive row of a visited (window, group) block still occupies MMA rows.
+// MMAs).  There are no global atomics and the result is deterministic, but where few windows
+// make the group range split over CTAs (see the host side): those add their fp32 partial sums
+// in any order, which more than two parts can show in the last bits.  The price is that an inactive
+// row of a visited (window, group) block still occupies MMA rows.
 //
 // Warp roles (320 threads):
 //   warps 0-3  epilogue: TMEM -> registers -> half -> global rows

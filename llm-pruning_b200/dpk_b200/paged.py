@@ -134,8 +134,9 @@ def attention_paged(Q: torch.Tensor, K_pages: torch.Tensor, V_pages: torch.Tenso
     It chooses between the kernel for a few tokens per sequence and the one for chunks, so give 1
     for a decode step; a larger sequence than it says is still computed, only slower.
 
-    Positions that hold no token may contain anything; what the new tokens themselves wrote as
-    values has to be finite."""
+    Head sizes 64 and 128, ``scale`` above zero.  Positions that hold no token may contain anything; what
+    the new tokens themselves wrote as values has to be finite.  Rows that see a score of NaN or +inf, or
+    scores of -inf alone, are NaN."""
     dev = _on_gpu(Q, K_pages, V_pages, page_table, kv_lens, query_start, Mask, O)
     code = _code(Q)
     if K_pages.dtype != Q.dtype:

@@ -260,7 +260,8 @@ class PagedKVCache:
                execute_attn: Optional[torch.Tensor] = None, scaling: Optional[float] = None,
                is_causal: bool = True, max_query_len: Optional[int] = None,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """:func:`routed_attention` of the new tokens ``[N,Hq,D]`` over everything cached of their sequence;
+        """:func:`routed_attention` of the new tokens ``[N,Hq,D]`` (D 64 or 128; the rest of the cache takes
+        any multiple of 16 up to 1024) over everything cached of their sequence;
         ``execute_attn [N,groups]`` (or ``[N]``) 0/1 of any dtype, ``None`` = every head."""
         if execute_attn is not None and execute_attn.dim() == 1:
             execute_attn = execute_attn[:, None]

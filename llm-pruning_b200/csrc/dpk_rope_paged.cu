@@ -206,10 +206,13 @@ __global__ void __launch_bounds__(kRopeWarps * 32, 5) rope_paged_kernel(const Ro
     // starts that no token looked at: sequences without a row, a first start that is not 0
     if (p.v) {
         const int64_t all = static_cast<int64_t>(gridDim.x) * (kRopeWarps * 32);
+        bool bad = false;
+#pragma unroll 8
         for (int64_t s = static_cast<int64_t>(blockIdx.x) * (kRopeWarps * 32) + threadIdx.x; s < p.S; s += all) {
             const int begin = p.qstart[s], end = p.qstart[s + 1];
-            if (begin < 0 || end < begin || end > p.N || (s == 0 && begin != 0)) rope_report(p);
+            bad |= begin < 0 || end < begin || end > p.N || (s == 0 && begin != 0);
         }
+        if (bad) rope_report(p);
     }
 }
 
